@@ -82,6 +82,20 @@ TRAIN_EXPORTS = ["swarm_lstm_seq_forward", "swarm_lstm_seq_backward", "swarm_rsa
                  "swarm_oc2_termination_terms_backward", "swarm_oc2_option_terms", "swarm_oc2_attention_terms",
                  "swarm_oc2_attention_terms_backward", "swarm_oc2_action_terms", "swarm_oc2_action_terms_backward",
                  "swarm_wgrad"]
+# Every symbol include/swarmseq.h declares (sequence-policy operators, same library).
+SEQ_EXPORTS = ["swarm_gated_scan_workspace", "swarm_gated_scan_forward", "swarm_gated_scan_backward",
+               "swarm_gated_step", "swarm_residual_norm_workspace", "swarm_residual_norm_forward",
+               "swarm_residual_norm_backward", "swarm_log_probs", "swarm_policy_loss_forward",
+               "swarm_policy_loss_backward"]
+GATED_TILE = 1                       # SWARM_GATED_TILE (include/swarmseq.h)
+POLICY_LOSS_PARTIALS = 2048 * 6      # SWARM_POLICY_LOSS_PARTIALS (include/swarmseq.h)
+
+
+def gated_tiles(steps: int) -> int:
+    """SWARM_GATED_TILES(T) (include/swarmseq.h)."""
+    return -(-steps // GATED_TILE)
+
+
 NORM_WIDTHS = (128, 256)   # row widths of swarm_row_norm_* / swarm_set_pool_*
 LSTM_MAX_BATCH = 6     # SWARM_LSTM_MAX_BATCH (include/swarmtrain.h)
 OC2_PARTIALS_FLOATS = 2048 * 24   # SWARM_OC2_PARTIALS_FLOATS (include/swarmtrain.h)
@@ -254,6 +268,26 @@ def load() -> C.CDLL:
     lib.swarm_oc2_attention_terms_backward.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
     lib.swarm_categorical_terms_backward.restype = i32
     lib.swarm_categorical_terms_backward.argtypes = [i64, i32, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.swarm_gated_scan_workspace.restype = i64
+    lib.swarm_gated_scan_workspace.argtypes = [i64, i64, i64]
+    lib.swarm_gated_scan_forward.restype = i32
+    lib.swarm_gated_scan_forward.argtypes = [i32, i64, i64, i64, vp, i64, i64] + [vp] * 8
+    lib.swarm_gated_scan_backward.restype = i32
+    lib.swarm_gated_scan_backward.argtypes = [i32, i64, i64, i64, vp, i64, i64, vp, vp, vp, vp, i64, i64] + [vp] * 5
+    lib.swarm_gated_step.restype = i32
+    lib.swarm_gated_step.argtypes = [i32, i64, i64, vp, i64] + [vp] * 5
+    lib.swarm_residual_norm_workspace.restype = i64
+    lib.swarm_residual_norm_workspace.argtypes = [i64, i64]
+    lib.swarm_residual_norm_forward.restype = i32
+    lib.swarm_residual_norm_forward.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, f32, vp, vp, vp, vp]
+    lib.swarm_residual_norm_backward.restype = i32
+    lib.swarm_residual_norm_backward.argtypes = [i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp, vp]
+    lib.swarm_log_probs.restype = i32
+    lib.swarm_log_probs.argtypes = [i32, i64, i64, vp, i64] + [vp] * 5
+    lib.swarm_policy_loss_forward.restype = i32
+    lib.swarm_policy_loss_forward.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6 + [f32] * 4 + [vp] * 7
+    lib.swarm_policy_loss_backward.restype = i32
+    lib.swarm_policy_loss_backward.argtypes = [i32, i64, i64, vp, i64, vp, f32] + [vp] * 5
     if lib.swarm_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libswarmstep ABI {lib.swarm_abi_version()} != expected {ABI_VERSION}")
     _lib = lib

@@ -12,7 +12,11 @@ from .learned_option_critic_networks import LearnedOptionActor, SquashedNormal
 from .option_critic_buffer import FixedOptionRolloutBuffer
 from .option_critic_networks import FixedOptionManager
 from .poca_buffer import POCARolloutBuffer
+from .sequence_ops import (categorical_log_probs, categorical_policy_loss, gated_recurrence, gated_recurrence_step,
+                           residual_rms_norm)
 
 __all__ = ["DecisionRecorder", "POCARolloutCollector", "POCAConfig", "FixedOptionCriticConfig",
            "LearnedOptionCriticConfig", "apply_network_settings", "load_config", "make_env_cfg", "POCARolloutBuffer", "FixedOptionRolloutBuffer", "LearnedOptionRolloutBuffer",
-           "FixedOptionManager", "LearnedOptionActor", "SquashedNormal", "poca_checkpoint", "save_poca_checkpoint", "load_poca_checkpoint", "actor_from_checkpoint", "evaluate"]
+           "FixedOptionManager", "LearnedOptionActor", "SquashedNormal", "poca_checkpoint", "save_poca_checkpoint", "load_poca_checkpoint", "actor_from_checkpoint", "evaluate",
+           "gated_recurrence", "gated_recurrence_step", "residual_rms_norm", "categorical_policy_loss",
+           "categorical_log_probs"]

@@ -1,0 +1,226 @@
+"""Sequence-policy operators without a GPU: the CPU form against the 64-bit reference, gradients against
+differences, every refusal (of the Python entry points and of the C ABI), and the header against the binding."""
+
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+import sequence_reference as R
+from conftest import ROOT
+from SwarmACB_isaac import _native
+from SwarmACB_isaac.agents import (categorical_log_probs, categorical_policy_loss, gated_recurrence,
+                                   gated_recurrence_step, residual_rms_norm)
+
+
+def _randn(*shape, seed=0, dtype=torch.float64):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=dtype)
+
+
+def _text():
+    return re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "swarmseq.h")).read(), flags=re.S)
+
+
+def test_header_and_binding_agree():
+    assert sorted(set(re.findall(r"\b(swarm_[a-z0-9_]+)\s*\(", _text()))) == sorted(_native.SEQ_EXPORTS)
+    lib = _native.load()
+    for name in _native.SEQ_EXPORTS:
+        assert hasattr(lib, name), name
+
+
+def test_header_constants_agree():
+    tile = int(re.search(r"#define SWARM_GATED_TILE (\d+)", _text()).group(1))
+    partials = re.search(r"#define SWARM_POLICY_LOSS_PARTIALS \((\d+) \* (\d+)\)", _text())
+    assert tile == _native.GATED_TILE
+    assert int(partials.group(1)) * int(partials.group(2)) == _native.POLICY_LOSS_PARTIALS
+    assert _native.gated_tiles(1) == 1 and _native.gated_tiles(tile) == 1 and _native.gated_tiles(tile + 1) == 2
+
+
+@pytest.mark.parametrize("n,T,U,with_keep,with_lengths", [(1, 1, 1, False, False), (3, 7, 5, True, False),
+                                                          (4, 9, 3, True, True), (2, 6, 4, False, True)])
+def test_recurrence_cpu(n, T, U, with_keep, with_lengths):
+    gates = _randn(n, T, 3 * U, seed=1).requires_grad_()
+    state = _randn(n, U, seed=2).requires_grad_()
+    keep = (torch.arange(n * T).view(n, T) % 3 != 1).double() if with_keep else None
+    lengths = torch.tensor([0, T, T // 2, 1])[:n] if with_lengths else None
+    d_h, d_last = _randn(n, T, U, seed=3), _randn(n, U, seed=4)
+    h, last = gated_recurrence(gates, state, keep, lengths)
+    grads = torch.autograd.grad((h, last), (gates, state), (d_h, d_last))
+    ref = R.recurrence(gates, state, keep, lengths, d_h, d_last)
+    for got, name in zip((h, last) + grads, ("h", "last", "d_gates", "d_state")):
+        R.check(got, ref[name][0], 1e-13 * (1 + ref[name][0].abs()), name)
+
+
+def test_recurrence_gradient_by_differences():
+    keep = torch.tensor([[1.0, 0.0, 1.0, 1.0], [1.0, 1.0, 1.0, 0.0]], dtype=torch.float64)
+    lengths = torch.tensor([4, 3])
+    gates, state = _randn(2, 4, 6, seed=5).requires_grad_(), _randn(2, 2, seed=6).requires_grad_()
+    assert torch.autograd.gradcheck(lambda g, s: gated_recurrence(g, s, keep, lengths), (gates, state))
+
+
+def test_recurrence_of_steps():
+    gates, state = _randn(3, 5, 12, seed=7), _randn(3, 4, seed=8)
+    keep = (torch.arange(15).view(3, 5) % 4 != 2).double()
+    h, last = gated_recurrence(gates, state, keep)
+    c = state
+    for t in range(5):
+        ht, c = gated_recurrence_step(gates[:, t], c, keep[:, t - 1] if t else None)
+        assert torch.allclose(ht, h[:, t], atol=1e-14)
+    assert torch.allclose(c, last, atol=1e-14)
+    buf = state.clone()
+    _, out = gated_recurrence_step(gates[:, 0], buf, inplace=True)
+    assert out is buf and not torch.equal(buf, state)
+
+
+@pytest.mark.parametrize("T,n", [(0, 3), (4, 0), (0, 0)])
+def test_recurrence_of_nothing(T, n):
+    state = _randn(n, 2, seed=9)
+    h, last = gated_recurrence(_randn(n, T, 6), state)
+    assert h.shape == (n, T, 2) and torch.equal(last, state)
+    assert last.data_ptr() != state.data_ptr() or n == 0
+
+
+@pytest.mark.parametrize("with_res,with_w", [(True, True), (False, True), (True, False), (False, False)])
+def test_norm_cpu(with_res, with_w):
+    x = _randn(3, 2, 7, seed=10).requires_grad_()
+    r = _randn(3, 2, 7, seed=11).requires_grad_() if with_res else None
+    w = _randn(7, seed=12).requires_grad_() if with_w else None
+    inputs = [t for t in (x, r, w) if t is not None]
+    assert torch.autograd.gradcheck(lambda *a: residual_rms_norm(x, r, w, eps=1e-3), inputs)
+    d_y, d_s = _randn(3, 2, 7, seed=13), _randn(3, 2, 7, seed=14)
+    y, s = residual_rms_norm(x, r, w, eps=1e-3)
+    ref = R.norm(x, r, w, 1e-3, d_y, d_s)
+    grads = dict(zip(("dx", "dr", "dw")[:1] + (("dr",) if with_res else ()) + (("dw",) if with_w else ()),
+                     torch.autograd.grad((y, s), inputs, (d_y, d_s))))
+    R.check(y, ref["y"][0], 1e-13 * (1 + ref["y"][0].abs()), "y")
+    for name, got in grads.items():
+        v = ref["dx" if name == "dr" else name][0]
+        R.check(got, v, 1e-13 * (1 + v.abs()), name)
+
+
+def _loss_inputs(M, K, seed=20):
+    z = 2 * _randn(M, K, seed=seed)
+    a = torch.randint(0, K, (M,), generator=torch.Generator().manual_seed(seed + 1))
+    l = torch.log_softmax(z, 1).gather(1, a[:, None])[:, 0]
+    return z, a, l - 0.3 * _randn(M, seed=seed + 2), _randn(M, seed=seed + 3), l + 0.3 * _randn(M, seed=seed + 4)
+
+
+@pytest.mark.parametrize("K", [1, 2, 6, 70])
+@pytest.mark.parametrize("kind", ["plain", "mask", "none active", "denom"])
+def test_policy_loss_cpu(K, kind):
+    M = 12
+    z, a, old, adv, ref = _loss_inputs(M, K)
+    if K > 2:
+        z[:, 1] = -torch.inf                    # a choice that cannot be taken
+        a[a == 1] = 0
+        old, ref = torch.log_softmax(z, 1).gather(1, a[:, None])[:, 0] + 0.25, old.clone()
+    mask = None if kind == "plain" else torch.arange(M) % 3 != 0 if kind != "none active" else torch.zeros(M, dtype=torch.bool)
+    denom = torch.tensor(7.0, dtype=torch.float64) if kind == "denom" else None
+    z.requires_grad_()
+    loss, terms = categorical_policy_loss(z, a, old, adv, clip=(0.1, 0.3), ref_log_probs=ref, kl_coef=0.2,
+                                          entropy_coef=0.05, mask=mask, denom=denom)
+    (d,) = torch.autograd.grad(loss, z)
+    want = R.policy_loss(z, a, old, adv, ref, mask, denom, 0.9, 1.3, 0.2, 0.05)
+    for got, name in ((loss, "loss"), (terms, "terms"), (d, "d_logits")):
+        R.check(got, want[name][0], 1e-12 * (1 + want[name][0].abs()), name)
+    lp, ent = categorical_log_probs(z.detach(), a)
+    l, _, H, _, _, _ = R.rows_of(z, a)
+    R.check(lp, l, 1e-12 * (1 + l.abs()), "log_probs")
+    R.check(ent, H, 1e-12 * (1 + H.abs()), "entropy")
+
+
+def test_policy_loss_gradient_by_differences():
+    z, a, old, adv, ref = _loss_inputs(5, 6)
+    mask = torch.tensor([True, True, False, True, True])
+    z.requires_grad_()
+    assert torch.autograd.gradcheck(
+        lambda q: categorical_policy_loss(q, a, old, adv, ref_log_probs=ref, kl_coef=0.3, entropy_coef=0.1, mask=mask)[0], (z,))
+
+
+def test_refusals():
+    f = torch.zeros
+    bad = [
+        lambda: gated_recurrence(f(2, 3, 7)), lambda: gated_recurrence(f(2, 6)), lambda: gated_recurrence(f(2, 3, 0)),
+        lambda: gated_recurrence(torch.zeros(2, 3, 6, dtype=torch.int32)),
+        lambda: gated_recurrence(f(2, 3, 6), f(2, 3)), lambda: gated_recurrence(f(2, 3, 6), f(2, 2).half()),
+        lambda: gated_recurrence(f(2, 3, 6), keep=f(2, 2)), lambda: gated_recurrence(f(2, 3, 6), keep=f(2, 3).int()),
+        lambda: gated_recurrence(f(2, 3, 6), keep=f(2, 3).requires_grad_()),
+        lambda: gated_recurrence(f(2, 3, 6), lengths=f(2)), lambda: gated_recurrence(f(2, 3, 6), lengths=[3, 3]),
+        lambda: gated_recurrence_step(f(2, 7), f(2, 2)), lambda: gated_recurrence_step(f(2, 6), None),
+        lambda: gated_recurrence_step(f(2, 6), f(2, 3)), lambda: gated_recurrence_step(f(2, 6).requires_grad_(), f(2, 2)),
+        lambda: gated_recurrence_step(f(2, 6), f(2, 4)[:, ::2], inplace=True),
+        lambda: residual_rms_norm(f(2, 0)), lambda: residual_rms_norm(f(())), lambda: residual_rms_norm(f(2, 4), f(4)),
+        lambda: residual_rms_norm(f(2, 4), f(2, 4).half()), lambda: residual_rms_norm(f(2, 4), weight=f(3)),
+        lambda: residual_rms_norm(f(2, 4), eps=-1.0), lambda: residual_rms_norm(f(2, 4), eps=float("nan")),
+        lambda: residual_rms_norm(torch.zeros(2, 4, dtype=torch.int64)),
+        lambda: categorical_log_probs(f(2, 0), f(2).long()), lambda: categorical_log_probs(f(2, 3), f(3).long()),
+        lambda: categorical_log_probs(f(2, 3), f(2)), lambda: categorical_log_probs(f(2, 3), None),
+        lambda: categorical_log_probs(f(2, 3).requires_grad_(), f(2).long()),
+    ]
+    loss = lambda z=f(2, 3), a=f(2).long(), o=f(2), v=f(2), **kw: categorical_policy_loss(z, a, o, v, **kw)  # noqa: E731
+    bad += [
+        lambda: loss(a=f(2)), lambda: loss(o=f(3)), lambda: loss(o=None), lambda: loss(v=None), lambda: loss(v=f(2).half()),
+        lambda: loss(o=f(2).requires_grad_()), lambda: loss(v=f(2).requires_grad_()), lambda: loss(mask=f(2)),
+        lambda: loss(mask=f(3).bool()), lambda: loss(denom=f(2)), lambda: loss(denom=3.0), lambda: loss(clip=(-0.5, -0.6)),
+        lambda: loss(clip=float("nan")), lambda: loss(kl_coef=0.1), lambda: loss(z=f(2, 0)),
+        lambda: loss(ref_log_probs=f(2, 1)), lambda: loss(ref_log_probs=f(2).requires_grad_()),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError(f"call {i} was not refused")
+
+
+def test_c_abi_refusals():
+    """The C entry points check before they touch the device: these return without one."""
+    lib = _native.load()
+    p = C.c_void_p(4096)            # never read: every call below is refused or has nothing to do
+    fwd = lambda dt=0, n=1, T=1, U=1, g=p, gn=3, gt=3, h=p, last=p: lib.swarm_gated_scan_forward(  # noqa: E731
+        dt, n, T, U, g, gn, gt, None, None, None, h, last, None, None, None)
+    assert fwd(n=0, g=None, h=None, last=None) == 0
+    for kw in (dict(dt=3), dict(dt=-1), dict(n=-1), dict(T=0), dict(U=0), dict(g=None), dict(h=None), dict(last=None),
+               dict(gn=-1), dict(gt=-1), dict(n=1 << 40, T=1 << 30), dict(U=1 << 60)):
+        assert fwd(**kw) == -1, kw
+    bwd = lambda dt=0, n=1, T=1, U=1, g=p, tiles=p, dg=p, hn=1: lib.swarm_gated_scan_backward(  # noqa: E731
+        dt, n, T, U, g, 3, 3, None, None, tiles, p, hn, 1, None, dg, None, None, None)
+    assert bwd(n=0) == 0
+    for kw in (dict(dt=9), dict(n=-1), dict(T=0), dict(U=0), dict(g=None), dict(tiles=None), dict(dg=None), dict(hn=-1)):
+        assert bwd(**kw) == -1, kw
+    step = lambda dt=0, rows=1, U=1, g=p, c=p, h=p, out=p, gr=3: lib.swarm_gated_step(  # noqa: E731
+        dt, rows, U, g, gr, c, None, h, out, None)
+    assert step(rows=0) == 0
+    for kw in (dict(dt=5), dict(rows=-1), dict(U=0), dict(g=None), dict(c=None), dict(h=None), dict(out=None), dict(gr=-1)):
+        assert step(**kw) == -1, kw
+    nf = lambda dt=0, rows=1, D=1, x=p, r=p, y=p, s=p, eps=1e-6: lib.swarm_residual_norm_forward(  # noqa: E731
+        dt, rows, D, x, 1, r, 1, None, eps, y, s, None, None)
+    assert nf(rows=0) == 0
+    for kw in (dict(dt=4), dict(rows=-1), dict(D=0), dict(x=None), dict(y=None), dict(s=None), dict(eps=-1.0),
+               dict(eps=float("nan")), dict(rows=1 << 40, D=1 << 30)):
+        assert nf(**kw) == -1, kw
+    nb = lambda dt=0, rows=1, D=1, s=p, rstd=p, dy=p, dx=p, dw=p, work=p: lib.swarm_residual_norm_backward(  # noqa: E731
+        dt, rows, D, s, 1, None, rstd, dy, 1, None, 0, dx, dw, work, None)
+    assert nb(rows=0, dw=None, work=None) == 0
+    for kw in (dict(dt=4), dict(rows=-1), dict(D=0), dict(s=None), dict(rstd=None), dict(dy=None), dict(dx=None),
+               dict(work=None)):
+        assert nb(**kw) == -1, kw
+    assert lib.swarm_residual_norm_workspace(-1, 4) == -1 and lib.swarm_residual_norm_workspace(4, 0) == -1
+    assert lib.swarm_gated_scan_workspace(0, 5, 5) >= 0
+    lp = lambda dt=0, M=1, K=1, z=p, a=p, o=p, e=p, ld=1: lib.swarm_log_probs(dt, M, K, z, ld, a, o, e, None, None)  # noqa: E731
+    assert lp(M=0) == 0
+    for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(o=None), dict(e=None), dict(ld=-1)):
+        assert lp(**kw) == -1, kw
+    lf = lambda dt=0, M=1, K=1, z=p, a=p, old=p, adv=p, lo=0.8, hi=1.2, loss=p, terms=p, used=p, st=p, part=p: (  # noqa: E731
+        lib.swarm_policy_loss_forward(dt, M, K, z, 1, a, old, None, adv, None, None, lo, hi, 0.0, 0.0, loss, terms,
+                                      used, st, part, None, None))
+    for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(old=None), dict(adv=None),
+               dict(lo=1.3), dict(lo=float("nan")), dict(loss=None), dict(terms=None), dict(used=None), dict(st=None),
+               dict(part=None)):
+        assert lf(**kw) == -1, kw
+    lb = lambda dt=0, M=1, K=1, z=p, a=p, st=p, used=p, g=p, d=p: lib.swarm_policy_loss_backward(  # noqa: E731
+        dt, M, K, z, 1, a, 0.0, st, used, g, d, None)
+    assert lb(M=0) == 0
+    for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(st=None), dict(used=None),
+               dict(g=None), dict(d=None)):
+        assert lb(**kw) == -1, kw
