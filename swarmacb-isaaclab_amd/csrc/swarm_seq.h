@@ -28,6 +28,37 @@ __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * -kLog2e));
 }
 
+// 16 bytes of elements at any address: global loads and stores of 16 bytes need no alignment on gfx950, so rows
+// of odd width and unaligned views take the same path. `valid` < V at the end of a row goes element by element.
+template <typename T>
+struct Pack {
+    static constexpr int V = 16 / sizeof(T);
+    T e[V];
+};
+
+template <typename T>
+__device__ __forceinline__ Pack<T> load_pack(const T* __restrict__ p, int valid) {
+    Pack<T> r;
+    if (valid >= Pack<T>::V) {
+        __builtin_memcpy(&r, p, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < Pack<T>::V; ++j) r.e[j] = j < valid ? p[j] : (T)0.0f;
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_pack(T* __restrict__ p, const Pack<T>& v, int valid) {
+    if (valid >= Pack<T>::V) {
+        __builtin_memcpy(p, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < Pack<T>::V; ++j)
+            if (j < valid) p[j] = v.e[j];
+    }
+}
+
 // Calls fn with a value of the element type that `dtype` names; false for an unknown dtype.
 template <typename F>
 bool with_type(int32_t dtype, F&& fn) {
