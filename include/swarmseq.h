@@ -42,7 +42,7 @@ typedef enum {
  *   h: [n][T][U]; c_last: [n][U] f32, the state behind the last step;
  *   tile_states: [n][SWARM_GATED_TILES(T)][U] f32, the state before every SWARM_GATED_TILE-th step, for the
  *   backward pass (NULL: not kept); work: swarm_gated_scan_workspace(n, T, U) floats (NULL where that is 0). */
-#define SWARM_GATED_TILE 128
+#define SWARM_GATED_TILE 32
 #define SWARM_GATED_TILES(T) (((int64_t)(T) + SWARM_GATED_TILE - 1) / SWARM_GATED_TILE)
 int64_t swarm_gated_scan_workspace(int64_t n, int64_t T, int64_t U);
 int32_t swarm_gated_scan_forward(int32_t dtype, int64_t n, int64_t T, int64_t U, const void* gates, int64_t gates_n,

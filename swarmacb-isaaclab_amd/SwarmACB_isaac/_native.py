@@ -87,7 +87,7 @@ SEQ_EXPORTS = ["swarm_gated_scan_workspace", "swarm_gated_scan_forward", "swarm_
                "swarm_gated_step", "swarm_residual_norm_workspace", "swarm_residual_norm_forward",
                "swarm_residual_norm_backward", "swarm_log_probs", "swarm_policy_loss_forward",
                "swarm_policy_loss_backward"]
-GATED_TILE = 128                     # SWARM_GATED_TILE (include/swarmseq.h)
+GATED_TILE = 32                      # SWARM_GATED_TILE (include/swarmseq.h)
 POLICY_LOSS_PARTIALS = 2048 * 6      # SWARM_POLICY_LOSS_PARTIALS (include/swarmseq.h)
 
 

@@ -16,6 +16,8 @@
 //
 // Few channels (one long sequence) do not fill the card: then the length is split into chunks as well, a first
 // kernel composes each chunk, and the main kernel's workgroups start from the chunks before theirs.
+#include <type_traits>
+
 #include "swarm_seq.h"
 
 using namespace swarm_seq;
@@ -24,16 +26,18 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChannels = 64;                  // channels of a workgroup
-constexpr int kTile = SWARM_GATED_TILE;        // steps of a tile
+constexpr int kTile = SWARM_GATED_TILE;        // steps of a tile of the backward pass, and between saved states
+constexpr int kFwdTile = 64;                   // steps of a tile of the forward pass
+static_assert(kFwdTile % kTile == 0, "the forward pass saves a state at segment starts");
 constexpr int kQuarters = kThreads / kChannels;   // threads that join one channel's segments
-constexpr int64_t kFill = 1024;                // workgroups that fill the card (four on each of 256 CUs)
+constexpr int64_t kFill = 512;                 // workgroups that fill the card (two on each of 256 CUs)
 
-template <typename T>
+template <int VV, int TILE>
 struct Shape {
-    static constexpr int V = Pack<T>::V;               // channels of a group
+    static constexpr int V = VV;                       // channels of a group
     static constexpr int kGroups = kChannels / V;      // groups of a workgroup
     static constexpr int kSegs = kThreads / kGroups;   // segments of a tile
-    static constexpr int kSteps = kTile / kSegs;       // steps of a segment
+    static constexpr int kSteps = TILE / kSegs;       // steps of a segment
     static constexpr int kPart = kSegs / kQuarters;    // segments that one joining thread composes
 };
 
@@ -44,55 +48,94 @@ struct ScanArgs {
     const float* keep;
     const int64_t* lengths;
     int64_t groups;        // groups of channels in each sequence
+    int64_t blocks;        // workgroups that hold all groups
     int64_t chunk_tiles;   // tiles of a chunk
     int64_t chunks;
     float* agg;            // [chunks][2][n][U]: a chunk's A and B
 };
 
-// What a thread works on: a group of channels of one sequence.
+// What a thread works on: V channels of one sequence, from u on. The last group of a sequence starts at U - V, so
+// that no vector load crosses a row's end: it may share channels with the one before, and both write the same.
+// Threads behind the last group read what the last group reads, and write nothing.
 struct Lane {
     int64_t i, u, len;
-    int valid;             // channels of the group that exist
+    bool exists;
 };
 
-template <typename T>
+template <int V>
 __device__ __forceinline__ Lane lane_of(const ScanArgs& p, int64_t group) {
     Lane l;
+    l.exists = group < p.n * p.groups;
+    if (!l.exists) group = p.n * p.groups - 1;
     l.i = group / p.groups;
-    l.u = (group - l.i * p.groups) * Pack<T>::V;
-    l.valid = 0;
-    l.len = 0;
-    if (l.i < p.n) {
-        l.valid = p.U - l.u < Pack<T>::V ? (int)(p.U - l.u) : Pack<T>::V;
-        l.len = p.lengths ? p.lengths[l.i] : p.steps;
-        if (l.len > p.steps) l.len = p.steps;
-    }
+    l.u = (group - l.i * p.groups) * V;
+    if (l.u > p.U - V) l.u = p.U - V;
+    l.len = p.lengths ? p.lengths[l.i] : p.steps;
+    if (l.len > p.steps) l.len = p.steps;
+    if (l.len < 0) l.len = 0;
     return l;
 }
 
-// keep before step t
-__device__ __forceinline__ float keep_of(const ScanArgs& p, int64_t i, int64_t t) {
-    return p.keep && t > 0 ? p.keep[i * p.steps + t - 1] : 1.0f;
-}
+// A thread's steps of one tile: R of the gate blocks (block r at column off[r]), with DH the gradient of h, and
+// keep before each step. Steps behind the end read the last one again (step 0 of an empty sequence): no load is
+// conditional, so all of them are in flight together, and their values are selected away.
+template <typename T, int V, int kSteps, int R, bool DH>
+struct Rows {
+    Pack<T, V> x[R][kSteps];
+    Pack<T, V> d[DH ? kSteps : 1];
+    float keep[kSteps];
+
+    __device__ __forceinline__ void load(const ScanArgs& p, const Lane& l, const T* g, const int64_t (&off)[R],
+                                         const T* dh, int64_t dt, int64_t t0) {
+        const int64_t end = l.len > 0 ? l.len - 1 : 0;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int64_t t = t0 + s < end ? t0 + s : end;
+            const T* q = g + t * p.gt;
+#pragma unroll
+            for (int r = 0; r < R; ++r) x[r][s].load(q + off[r]);
+            if (DH) d[s].load(dh + t * dt);
+            keep[s] = p.keep ? p.keep[l.i * p.steps + (t > 0 ? t - 1 : 0)] : 1.0f;
+            if (t == 0) keep[s] = 1.0f;
+        }
+    }
+};
 
 __device__ __forceinline__ void compose(float& A, float& B, float a, float b) {
     B = a * B + b;
     A = a * A;
 }
 
+// The step that every sequence of the workgroup reaches.
+template <typename R>
+__device__ __forceinline__ int64_t whole_until(const ScanArgs& p, int64_t len, R& red) {
+    if (!p.lengths) return p.steps;
+    const int short_of = __syncthreads_or(len < p.steps);
+    if (!short_of) return p.steps;
+    int64_t* least = reinterpret_cast<int64_t*>(&red);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const int64_t other = __shfl_xor(len, o);
+        len = other < len ? other : len;
+    }
+    if (threadIdx.x % 64 == 0) least[threadIdx.x / 64] = len;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 64; ++w) len = least[w] < len ? least[w] : len;
+    __syncthreads();
+    return len;
+}
+
 // (A, B) of the chunks [from, to) in their order along the walk, by the joining threads of a channel, in every one
 __device__ __forceinline__ void chunks_before(const ScanArgs& p, int64_t at, int64_t first, int64_t count, int64_t dir,
-                                              int quarter, float (*red)[kChannels][2], int ch, bool exists, float& A,
-                                              float& B) {
+                                              int quarter, float (*red)[kChannels][2], int ch, float& A, float& B) {
     A = 1.0f;
     B = 0.0f;
     const int64_t size = p.n * p.U;
     const int64_t k0 = count * quarter / kQuarters, k1 = count * (quarter + 1) / kQuarters;
-    if (exists)
-        for (int64_t k = k0; k < k1; ++k) {
-            const float* a = p.agg + (first + dir * k) * 2 * size + at;
-            compose(A, B, a[0], a[size]);
-        }
+    for (int64_t k = k0; k < k1; ++k) {
+        const float* a = p.agg + (first + dir * k) * 2 * size + at;
+        compose(A, B, a[0], a[size]);
+    }
     red[quarter][ch][0] = A;
     red[quarter][ch][1] = B;
     __syncthreads();
@@ -103,140 +146,131 @@ __device__ __forceinline__ void chunks_before(const ScanArgs& p, int64_t at, int
 }
 
 // A chunk's composition. Forward: of c; backward (BWD): of E, from its last step to its first.
-template <typename T, bool BWD>
-__global__ __launch_bounds__(kThreads) void chunk_kernel(ScanArgs p, const T* __restrict__ dh, int64_t dn, int64_t dt) {
-    using S = Shape<T>;
-    __shared__ float ab[S::kSegs][kChannels][2];
-    __shared__ float red[kQuarters][kChannels][2];
-    const int64_t blocks = (p.n * p.groups + S::kGroups - 1) / S::kGroups;
-    const int64_t part = blockIdx.x / blocks, block = blockIdx.x - part * blocks;
+template <typename T, int V, bool BWD>
+__global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void chunk_kernel(ScanArgs p, const T* dh, int64_t dn, int64_t dt) {
+    using S = Shape<V, kFwdTile>;
+    __shared__ float ab[2][S::kSegs][kChannels];
+    __shared__ __align__(8) float red[kQuarters][kChannels][2];
+    const int64_t part = blockIdx.x / p.blocks, block = blockIdx.x - part * p.blocks;
     const int64_t chunk = BWD ? part + 1 : part;
     const int lane = threadIdx.x % S::kGroups, seg = threadIdx.x / S::kGroups;
-    const Lane l = lane_of<T>(p, block * S::kGroups + lane);
+    const Lane l = lane_of<V>(p, block * S::kGroups + lane);
     const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
+    const bool has_dh = BWD && dh;
+    const T* dhp = has_dh ? dh + l.i * dn + l.u : g;
     const int ch = threadIdx.x % kChannels, quarter = threadIdx.x / kChannels;
-    const Lane jl = lane_of<T>(p, block * S::kGroups + ch / S::V);
-    const bool exists = ch % S::V < jl.valid;
     float cA = 1.0f, cB = 0.0f;
+    const int64_t off[2] = {0, (BWD ? 2 : 1) * p.U};
+    auto start = [&](int64_t k) {      // the thread's first step of the walk's tile k
+        return (chunk * p.chunk_tiles + (BWD ? p.chunk_tiles - 1 - k : k)) * kFwdTile + seg * S::kSteps;
+    };
     for (int64_t k = 0; k < p.chunk_tiles; ++k) {
-        const int64_t tile = chunk * p.chunk_tiles + (BWD ? p.chunk_tiles - 1 - k : k);
-        const int64_t t0 = tile * kTile + seg * S::kSteps;
-        Pack<T> x[S::kSteps], y[S::kSteps], d[BWD ? S::kSteps : 1];
+        const int64_t t0 = start(k);
+        Rows<T, V, S::kSteps, 2, BWD> now;
+        now.load(p, l, g, off, dhp, dt, t0);
+        float A[V], B[V];
 #pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-            const int valid = t0 + s < l.len ? l.valid : 0;
-            x[s] = load_pack(g + (t0 + s) * p.gt, valid);
-            y[s] = load_pack(g + (t0 + s) * p.gt + (BWD ? 2 : 1) * p.U, valid);
-            if (BWD) d[s] = load_pack(dh + l.i * dn + (t0 + s) * dt + l.u, dh ? valid : 0);
-        }
-        float A[S::V], B[S::V];
-#pragma unroll
-        for (int j = 0; j < S::V; ++j) A[j] = 1.0f, B[j] = 0.0f;
+        for (int j = 0; j < V; ++j) A[j] = 1.0f, B[j] = 0.0f;
 #pragma unroll
         for (int q = 0; q < S::kSteps; ++q) {
             const int s = BWD ? S::kSteps - 1 - q : q;
-            if (t0 + s >= l.len) continue;
-            const float kp = keep_of(p, l.i, t0 + s);
+            const bool on = t0 + s < l.len;
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) {
-                float f, b;
-                sigmoid_pair((float)x[s].e[j], f, b);
-                const float a = f * kp;
-                compose(A[j], B[j], a, BWD ? a * (sigmoid((float)y[s].e[j]) * (float)d[s].e[j]) : b * (float)y[s].e[j]);
+            for (int j = 0; j < V; ++j) {
+                float f, m;
+                sigmoid_pair(now.x[0][s].get(j), f, m);
+                const float y = now.x[1][s].get(j), a = f * now.keep[s];
+                const float b = BWD ? a * (sigmoid(y) * (has_dh ? now.d[s].get(j) : 0.0f)) : m * y;
+                compose(A[j], B[j], on ? a : 1.0f, on ? b : 0.0f);
             }
         }
 #pragma unroll
-        for (int j = 0; j < S::V; ++j) {
-            ab[BWD ? S::kSegs - 1 - seg : seg][lane * S::V + j][0] = A[j];
-            ab[BWD ? S::kSegs - 1 - seg : seg][lane * S::V + j][1] = B[j];
+        for (int j = 0; j < V; ++j) {
+            ab[0][BWD ? S::kSegs - 1 - seg : seg][lane * V + j] = A[j];
+            ab[1][BWD ? S::kSegs - 1 - seg : seg][lane * V + j] = B[j];
         }
         __syncthreads();
         float qA = 1.0f, qB = 0.0f;
 #pragma unroll
-        for (int s = 0; s < S::kPart; ++s) {
-            const float* e = ab[quarter * S::kPart + s][ch];
-            compose(qA, qB, e[0], e[1]);
-        }
+        for (int s = 0; s < S::kPart; ++s)
+            compose(qA, qB, ab[0][quarter * S::kPart + s][ch], ab[1][quarter * S::kPart + s][ch]);
         red[quarter][ch][0] = qA;
         red[quarter][ch][1] = qB;
         __syncthreads();
         for (int q = 0; q < kQuarters; ++q) compose(cA, cB, red[q][ch][0], red[q][ch][1]);
     }
-    if (quarter == 0 && exists) {
-        float* out = p.agg + chunk * 2 * p.n * p.U + jl.i * p.U + jl.u + ch % S::V;
-        out[0] = cA;
-        out[p.n * p.U] = cB;
+    if (quarter == 0) {
+        const Lane jl = lane_of<V>(p, block * S::kGroups + ch / V);
+        float* out = p.agg + chunk * 2 * p.n * p.U + jl.i * p.U + jl.u + ch % V;
+        if (jl.exists) {
+            out[0] = cA;
+            out[p.n * p.U] = cB;
+        }
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p, const float* __restrict__ c0, T* __restrict__ h,
-                                                            float* __restrict__ c_last, float* __restrict__ states) {
-    using S = Shape<T>;
-    __shared__ float ab[S::kSegs][kChannels][2];
-    __shared__ float red[kQuarters][kChannels][2];
-    const int64_t blocks = (p.n * p.groups + S::kGroups - 1) / S::kGroups;
-    const int64_t chunk = blockIdx.x / blocks, block = blockIdx.x - chunk * blocks;
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(ScanArgs p, const float* __restrict__ c0, T* __restrict__ h,
+                                                               float* __restrict__ c_last,
+                                                               float* __restrict__ states) {
+    using S = Shape<V, kFwdTile>;
+    __shared__ float ab[2][S::kSegs][kChannels];
+    __shared__ __align__(8) float red[kQuarters][kChannels][2];
+    const int64_t chunk = blockIdx.x / p.blocks, block = blockIdx.x - chunk * p.blocks;
     const int lane = threadIdx.x % S::kGroups, seg = threadIdx.x / S::kGroups;
-    const Lane l = lane_of<T>(p, block * S::kGroups + lane);
+    const Lane l = lane_of<V>(p, block * S::kGroups + lane);
     const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
     const int ch = threadIdx.x % kChannels, quarter = threadIdx.x / kChannels;
-    const Lane jl = lane_of<T>(p, block * S::kGroups + ch / S::V);
-    const bool exists = ch % S::V < jl.valid;
-    const int64_t at = jl.i * p.U + jl.u + ch % S::V;
-    const int64_t tiles = (p.steps + kTile - 1) / kTile;
-    float carry = exists && c0 ? c0[at] : 0.0f;      // the channel's state before the tile, in every joining thread
-    if (chunk > 0) {
-        float A, B;
-        chunks_before(p, at, 0, chunk, 1, quarter, red, ch, exists, A, B);
-        carry = A * carry + B;
-    }
+    const Lane jl = lane_of<V>(p, block * S::kGroups + ch / V);
+    const int64_t at = jl.i * p.U + jl.u + ch % V;
+    const int64_t tiles = (p.steps + kFwdTile - 1) / kFwdTile;
+    const int64_t saved = SWARM_GATED_TILES(p.steps);
     const int64_t first = chunk * p.chunk_tiles;
     const int64_t last = first + p.chunk_tiles < tiles ? first + p.chunk_tiles : tiles;
-    for (int64_t tile = first; tile < last; ++tile) {
-        const int64_t t0 = tile * kTile + seg * S::kSteps;
-        Pack<T> xf[S::kSteps], xz[S::kSteps], xo[S::kSteps];
+    const int64_t off[3] = {0, p.U, 2 * p.U};
+    const int64_t whole = whole_until(p, l.len, red);
+    float carry = c0 ? c0[at] : 0.0f;      // the channel's state before the tile, in every joining thread
+    if (chunk > 0) {
+        float A, B;
+        chunks_before(p, at, 0, chunk, 1, quarter, red, ch, A, B);
+        carry = A * carry + B;
+    }
+    auto run = [&](int64_t tile, auto all) {
+        constexpr bool ALL = decltype(all)::value;      // no step of the tile is padding
+        const int64_t t0 = tile * kFwdTile + seg * S::kSteps;
+        Rows<T, V, S::kSteps, 3, false> rows;
+        rows.load(p, l, g, off, g, 0, t0);
+        float a[S::kSteps][V], b[S::kSteps][V], A[V], B[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) A[j] = 1.0f, B[j] = 0.0f;
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s) {
-            const int valid = t0 + s < l.len ? l.valid : 0;
-            const T* q = g + (t0 + s) * p.gt;
-            xf[s] = load_pack(q, valid);
-            xz[s] = load_pack(q + p.U, valid);
-            xo[s] = load_pack(q + 2 * p.U, valid);
-        }
-        float a[S::kSteps][S::V], b[S::kSteps][S::V], A[S::V], B[S::V];
+            const bool on = ALL || t0 + s < l.len;
 #pragma unroll
-        for (int j = 0; j < S::V; ++j) A[j] = 1.0f, B[j] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-            const bool on = t0 + s < l.len;
-            const float kp = on ? keep_of(p, l.i, t0 + s) : 1.0f;
-#pragma unroll
-            for (int j = 0; j < S::V; ++j) {
+            for (int j = 0; j < V; ++j) {
                 float f, m;
-                sigmoid_pair((float)xf[s].e[j], f, m);
-                a[s][j] = on ? f * kp : 1.0f;
-                b[s][j] = on ? m * (float)xz[s].e[j] : 0.0f;
+                sigmoid_pair(rows.x[0][s].get(j), f, m);
+                a[s][j] = on ? f * rows.keep[s] : 1.0f;
+                b[s][j] = on ? m * rows.x[1][s].get(j) : 0.0f;
                 compose(A[j], B[j], a[s][j], b[s][j]);
             }
         }
 #pragma unroll
-        for (int j = 0; j < S::V; ++j) {
-            ab[seg][lane * S::V + j][0] = A[j];
-            ab[seg][lane * S::V + j][1] = B[j];
+        for (int j = 0; j < V; ++j) {
+            ab[0][seg][lane * V + j] = A[j];
+            ab[1][seg][lane * V + j] = B[j];
         }
         __syncthreads();
         float pA[S::kPart], pB[S::kPart], qA = 1.0f, qB = 0.0f;
 #pragma unroll
         for (int s = 0; s < S::kPart; ++s) {
-            pA[s] = ab[quarter * S::kPart + s][ch][0];
-            pB[s] = ab[quarter * S::kPart + s][ch][1];
+            pA[s] = ab[0][quarter * S::kPart + s][ch];
+            pB[s] = ab[1][quarter * S::kPart + s][ch];
             compose(qA, qB, pA[s], pB[s]);
         }
         red[quarter][ch][0] = qA;
         red[quarter][ch][1] = qB;
         __syncthreads();
-        if (states && quarter == 0 && exists) states[(jl.i * tiles + tile) * p.U + jl.u + ch % S::V] = carry;
         float c = carry;
 #pragma unroll
         for (int q = 0; q < kQuarters; ++q) {
@@ -245,103 +279,106 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p, const fl
         }
 #pragma unroll
         for (int s = 0; s < S::kPart; ++s) {
-            ab[quarter * S::kPart + s][ch][0] = c;
+            const int first_step = (quarter * S::kPart + s) * S::kSteps;
+            if (states && first_step % kTile == 0 && jl.exists && tile * kFwdTile + first_step < p.steps)
+                states[(jl.i * saved + tile * (kFwdTile / kTile) + first_step / kTile) * p.U + jl.u + ch % V] = c;
+            ab[0][quarter * S::kPart + s][ch] = c;
             c = pA[s] * c + pB[s];
         }
         __syncthreads();
-        float now[S::V];
+        float now[V];
 #pragma unroll
-        for (int j = 0; j < S::V; ++j) now[j] = ab[seg][lane * S::V + j][0];
+        for (int j = 0; j < V; ++j) now[j] = ab[0][seg][lane * V + j];
         T* out = h + (l.i * p.steps + t0) * p.U + l.u;
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s) {
-            Pack<T> v;
-            const bool on = t0 + s < l.len;
+            float v[V];
+            const bool on = ALL || t0 + s < l.len;
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) {
+            for (int j = 0; j < V; ++j) {
                 now[j] = a[s][j] * now[j] + b[s][j];
-                v.e[j] = (T)(on ? sigmoid((float)xo[s].e[j]) * now[j] : 0.0f);
+                v[j] = on ? sigmoid(rows.x[2][s].get(j)) * now[j] : 0.0f;
             }
-            store_pack(out + s * p.U, v, t0 + s < p.steps ? l.valid : 0);
+            Pack<T, V> w;
+            w.set(v);
+            if (l.exists && (ALL || t0 + s < p.steps)) w.store(out + s * p.U);
         }
         __syncthreads();
+    };
+    for (int64_t tile = first; tile < last; ++tile) {
+        if ((tile + 1) * kFwdTile <= whole) run(tile, std::true_type{});
+        else run(tile, std::false_type{});
     }
-    if (chunk == p.chunks - 1 && quarter == 0 && exists) c_last[at] = carry;
+    if (chunk == p.chunks - 1 && quarter == 0 && jl.exists) c_last[at] = carry;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p, const float* __restrict__ states,
-                                                            const T* __restrict__ dh, int64_t dn, int64_t dt,
-                                                            const float* __restrict__ d_last, T* __restrict__ dg,
-                                                            float* __restrict__ d_c0) {
-    using S = Shape<T>;
-    __shared__ float ab[S::kSegs][kChannels][3];     // A, B and the gradient's B; then the states before and behind
-    __shared__ float red[kQuarters][kChannels][3];
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(ScanArgs p, const float* __restrict__ states, const T* dh,
+                                                               int64_t dn, int64_t dt,
+                                                               const float* __restrict__ d_last, T* __restrict__ dg,
+                                                               float* __restrict__ d_c0) {
+    using S = Shape<V, kTile>;
+    __shared__ float ab[3][S::kSegs][kChannels];     // A, B and the gradient's B; then the states before and behind
+    __shared__ __align__(8) float red[kQuarters][kChannels][3];
     float (*before)[kChannels][2] = reinterpret_cast<float (*)[kChannels][2]>(&red[0][0][0]);
-    const int64_t blocks = (p.n * p.groups + S::kGroups - 1) / S::kGroups;
-    const int64_t chunk = blockIdx.x / blocks, block = blockIdx.x - chunk * blocks;
+    const int64_t chunk = blockIdx.x / p.blocks, block = blockIdx.x - chunk * p.blocks;
     const int lane = threadIdx.x % S::kGroups, seg = threadIdx.x / S::kGroups;
-    const Lane l = lane_of<T>(p, block * S::kGroups + lane);
+    const Lane l = lane_of<V>(p, block * S::kGroups + lane);
     const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
-    const T* dhp = dh + l.i * dn + l.u;
+    const T* dhp = dh ? dh + l.i * dn + l.u : g;
     const int ch = threadIdx.x % kChannels, quarter = threadIdx.x / kChannels;
-    const Lane jl = lane_of<T>(p, block * S::kGroups + ch / S::V);
-    const bool exists = ch % S::V < jl.valid;
-    const int64_t at = jl.i * p.U + jl.u + ch % S::V;
+    const Lane jl = lane_of<V>(p, block * S::kGroups + ch / V);
+    const int64_t at = jl.i * p.U + jl.u + ch % V;
     const int64_t tiles = (p.steps + kTile - 1) / kTile;
-    float carry = exists && d_last ? d_last[at] : 0.0f;     // E behind the tile
+    const int64_t chunk_tiles = p.chunk_tiles * (kFwdTile / kTile), first = chunk * chunk_tiles;
+    const int64_t last = first + chunk_tiles < tiles ? first + chunk_tiles : tiles;
+    const int64_t off[3] = {0, p.U, 2 * p.U};
+    const int64_t whole = whole_until(p, l.len, red);
+    float carry = d_last ? d_last[at] : 0.0f;     // E behind the tile
     if (chunk < p.chunks - 1) {
         float A, B;
-        chunks_before(p, at, p.chunks - 1, p.chunks - 1 - chunk, -1, quarter, before, ch, exists, A, B);
+        chunks_before(p, at, p.chunks - 1, p.chunks - 1 - chunk, -1, quarter, before, ch, A, B);
         carry = A * carry + B;
     }
-    const int64_t first = chunk * p.chunk_tiles;
-    const int64_t last = first + p.chunk_tiles < tiles ? first + p.chunk_tiles : tiles;
-    for (int64_t tile = last - 1; tile >= first; --tile) {
+    auto run = [&](int64_t tile, auto all) {
+        constexpr bool ALL = decltype(all)::value;
         const int64_t t0 = tile * kTile + seg * S::kSteps;
-        Pack<T> xf[S::kSteps], xz[S::kSteps], xo[S::kSteps], d[S::kSteps];
-        float kp[S::kSteps];
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-            const int valid = t0 + s < l.len ? l.valid : 0;
-            const T* q = g + (t0 + s) * p.gt;
-            xf[s] = load_pack(q, valid);
-            xz[s] = load_pack(q + p.U, valid);
-            xo[s] = load_pack(q + 2 * p.U, valid);
-            d[s] = load_pack(dhp + (t0 + s) * dt, dh ? valid : 0);
-            kp[s] = t0 + s < l.len ? keep_of(p, l.i, t0 + s) : 1.0f;
-        }
-        const float start = exists ? states[(jl.i * tiles + tile) * p.U + jl.u + ch % S::V] : 0.0f;
+        const float start = states[(jl.i * tiles + tile) * p.U + jl.u + ch % V];
+        Rows<T, V, S::kSteps, 3, true> rows;
+        rows.load(p, l, g, off, dhp, dt, t0);
         {
-            float A[S::V], B[S::V], G[S::V];
+            float A[V], B[V], G[V];
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) A[j] = 1.0f, B[j] = 0.0f, G[j] = 0.0f;
+            for (int j = 0; j < V; ++j) A[j] = 1.0f, B[j] = 0.0f, G[j] = 0.0f;
 #pragma unroll
             for (int s = 0; s < S::kSteps; ++s) {
-                if (t0 + s >= l.len) continue;
+                const bool on = ALL || t0 + s < l.len;
 #pragma unroll
-                for (int j = 0; j < S::V; ++j) {
+                for (int j = 0; j < V; ++j) {
                     float f, m;
-                    sigmoid_pair((float)xf[s].e[j], f, m);
-                    const float a = f * kp[s];
-                    B[j] = a * B[j] + m * (float)xz[s].e[j];
+                    sigmoid_pair(rows.x[0][s].get(j), f, m);
+                    const float a = on ? f * rows.keep[s] : 1.0f;
+                    const float od = sigmoid(rows.x[2][s].get(j)) * (dh ? rows.d[s].get(j) : 0.0f);
+                    B[j] = a * B[j] + (on ? m * rows.x[1][s].get(j) : 0.0f);
                     A[j] *= a;
                     // E at the segment's first step is the sum of a_0 .. a_s (o dh)_s
-                    G[j] += A[j] * (sigmoid((float)xo[s].e[j]) * (float)d[s].e[j]);
+                    G[j] += on ? A[j] * od : 0.0f;
                 }
             }
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) {
-                float* e = ab[seg][lane * S::V + j];
-                e[0] = A[j], e[1] = B[j], e[2] = G[j];
+            for (int j = 0; j < V; ++j) {
+                ab[0][seg][lane * V + j] = A[j];
+                ab[1][seg][lane * V + j] = B[j];
+                ab[2][seg][lane * V + j] = G[j];
             }
         }
         __syncthreads();
         float pA[S::kPart], pB[S::kPart], pG[S::kPart], qA = 1.0f, qB = 0.0f, qG = 0.0f;
 #pragma unroll
         for (int s = 0; s < S::kPart; ++s) {
-            const float* e = ab[quarter * S::kPart + s][ch];
-            pA[s] = e[0], pB[s] = e[1], pG[s] = e[2];
+            pA[s] = ab[0][quarter * S::kPart + s][ch];
+            pB[s] = ab[1][quarter * S::kPart + s][ch];
+            pG[s] = ab[2][quarter * S::kPart + s][ch];
             qB = pA[s] * qB + pB[s];
             qG += qA * pG[s];
             qA *= pA[s];
@@ -361,60 +398,67 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p, const fl
         }
 #pragma unroll
         for (int s = 0; s < S::kPart; ++s) {
-            ab[quarter * S::kPart + s][ch][0] = c;
+            ab[0][quarter * S::kPart + s][ch] = c;
             c = pA[s] * c + pB[s];
         }
 #pragma unroll
         for (int s = S::kPart - 1; s >= 0; --s) {
-            ab[quarter * S::kPart + s][ch][1] = E;
+            ab[1][quarter * S::kPart + s][ch] = E;
             E = pA[s] * E + pG[s];
         }
         __syncthreads();
-        float now[S::V], back[S::V], cs[S::kSteps][S::V];
+        float now[V], back[V], cs[S::kSteps][V];
 #pragma unroll
-        for (int j = 0; j < S::V; ++j) {
-            now[j] = ab[seg][lane * S::V + j][0];
-            back[j] = ab[seg][lane * S::V + j][1];
+        for (int j = 0; j < V; ++j) {
+            now[j] = ab[0][seg][lane * V + j];
+            back[j] = ab[1][seg][lane * V + j];
         }
 #pragma unroll
         for (int s = 0; s < S::kSteps; ++s) {
-            const bool on = t0 + s < l.len;
+            const bool on = ALL || t0 + s < l.len;
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) {
+            for (int j = 0; j < V; ++j) {
                 float f, m;
-                sigmoid_pair((float)xf[s].e[j], f, m);
-                cs[s][j] = now[j] * kp[s];
-                now[j] = on ? f * cs[s][j] + m * (float)xz[s].e[j] : now[j];
+                sigmoid_pair(rows.x[0][s].get(j), f, m);
+                cs[s][j] = now[j] * rows.keep[s];
+                now[j] = on ? f * cs[s][j] + m * rows.x[1][s].get(j) : now[j];
             }
         }
         T* out = dg + (l.i * p.steps + t0) * 3 * p.U + l.u;
 #pragma unroll
         for (int s = S::kSteps - 1; s >= 0; --s) {
-            const bool on = t0 + s < l.len;
-            Pack<T> vf, vz, vo;
+            const bool on = ALL || t0 + s < l.len;
+            float vf[V], vz[V], vo[V];
 #pragma unroll
-            for (int j = 0; j < S::V; ++j) {
+            for (int j = 0; j < V; ++j) {
                 float f, m, o, om;
-                sigmoid_pair((float)xf[s].e[j], f, m);
-                sigmoid_pair((float)xo[s].e[j], o, om);
-                const float z = (float)xz[s].e[j], dd = (float)d[s].e[j], pr = cs[s][j];
+                sigmoid_pair(rows.x[0][s].get(j), f, m);
+                sigmoid_pair(rows.x[2][s].get(j), o, om);
+                const float z = rows.x[1][s].get(j), pr = cs[s][j];
                 const float cc = f * pr + m * z;
-                const float od = o * dd;
+                const float od = o * (dh ? rows.d[s].get(j) : 0.0f);
                 const float D = od + back[j];
-                vf.e[j] = (T)(on ? D * (pr - z) * (f * m) : 0.0f);
-                vz.e[j] = (T)(on ? D * m : 0.0f);
-                vo.e[j] = (T)(on ? od * om * cc : 0.0f);
-                back[j] = on ? f * kp[s] * D : back[j];
+                vf[j] = on ? D * (pr - z) * (f * m) : 0.0f;
+                vz[j] = on ? D * m : 0.0f;
+                vo[j] = on ? od * om * cc : 0.0f;
+                back[j] = on ? f * rows.keep[s] * D : back[j];
             }
-            const int valid = t0 + s < p.steps ? l.valid : 0;
             T* w = out + s * 3 * p.U;
-            store_pack(w, vf, valid);
-            store_pack(w + p.U, vz, valid);
-            store_pack(w + 2 * p.U, vo, valid);
+            Pack<T, V> wf, wz, wo;
+            wf.set(vf), wz.set(vz), wo.set(vo);
+            if (l.exists && (ALL || t0 + s < p.steps)) {
+                wf.store(w);
+                wz.store(w + p.U);
+                wo.store(w + 2 * p.U);
+            }
         }
         __syncthreads();
+    };
+    for (int64_t tile = last - 1; tile >= first; --tile) {
+        if ((tile + 1) * kTile <= whole) run(tile, std::true_type{});
+        else run(tile, std::false_type{});
     }
-    if (d_c0 && chunk == 0 && quarter == 0 && exists) d_c0[at] = carry;
+    if (d_c0 && chunk == 0 && quarter == 0 && jl.exists) d_c0[at] = carry;
 }
 
 template <typename T>
@@ -439,18 +483,28 @@ bool blocks_of(int64_t items, unsigned& blocks) {
     return b <= 0x7fffffff;
 }
 
-int64_t width_of(int32_t dtype) { return dtype == SWARM_F32 ? 4 : 8; }
+// Vectors of kWide channels; sequences narrower than that go channel by channel.
+constexpr int kWide = 4;
+int64_t width_of(int64_t U) { return U >= kWide ? kWide : 1; }
 
 // How the length is split: whole tiles, as many chunks as fill the card together with the channels.
-void split(int64_t n, int64_t T, int64_t U, int64_t V, int64_t& groups, int64_t& blocks, int64_t& chunk_tiles,
-           int64_t& chunks) {
-    groups = (U + V - 1) / V;
-    blocks = (n * groups + kChannels / V - 1) / (kChannels / V);
-    const int64_t tiles = SWARM_GATED_TILES(T);
-    int64_t want = blocks >= kFill ? 1 : (kFill + blocks - 1) / blocks;
+void split(ScanArgs& p) {
+    const int64_t V = width_of(p.U), per_block = kChannels / V;
+    p.groups = (p.U + V - 1) / V;
+    p.blocks = (p.n * p.groups + per_block - 1) / per_block;
+    const int64_t tiles = (p.steps + kFwdTile - 1) / kFwdTile;
+    int64_t want = p.blocks >= kFill ? 1 : (kFill + p.blocks - 1) / p.blocks;
     if (want > tiles) want = tiles;
-    chunk_tiles = (tiles + want - 1) / want;
-    chunks = (tiles + chunk_tiles - 1) / chunk_tiles;
+    p.chunk_tiles = (tiles + want - 1) / want;
+    p.chunks = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+}
+
+template <typename F>
+void with_type_and_width(int32_t dtype, int64_t U, F&& fn) {
+    with_type(dtype, [&](auto e) {
+        if (width_of(U) == kWide) fn(e, std::integral_constant<int, kWide>{});
+        else fn(e, std::integral_constant<int, 1>{});
+    });
 }
 
 }  // namespace
@@ -460,13 +514,9 @@ extern "C" {
 int64_t swarm_gated_scan_workspace(int64_t n, int64_t T, int64_t U) {
     if (n < 0 || T < 1 || U < 1 || !sane(n, T, U)) return SWARM_ERR_ARG;
     if (n == 0) return 0;
-    int64_t most = 0;
-    for (int64_t V : {4, 8}) {
-        int64_t groups, blocks, chunk_tiles, chunks;
-        split(n, T, U, V, groups, blocks, chunk_tiles, chunks);
-        if (chunks > most) most = chunks;
-    }
-    return most > 1 ? most * 2 * n * U : 0;
+    ScanArgs p{n, T, U};
+    split(p);
+    return p.chunks > 1 ? p.chunks * 2 * n * U : 0;
 }
 
 int32_t swarm_gated_scan_forward(int32_t dtype, int64_t n, int64_t T, int64_t U, const void* gates, int64_t gates_n,
@@ -475,17 +525,17 @@ int32_t swarm_gated_scan_forward(int32_t dtype, int64_t n, int64_t T, int64_t U,
     if (!known_type(dtype) || n < 0 || T < 1 || U < 1 || !sane(n, T, U)) return SWARM_ERR_ARG;
     if (n == 0) return SWARM_OK;
     if (!gates || !h || !c_last || gates_t < 0 || gates_n < 0) return SWARM_ERR_ARG;
-    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, work};
-    int64_t blocks;
-    split(n, T, U, width_of(dtype), p.groups, blocks, p.chunk_tiles, p.chunks);
-    if (blocks * p.chunks > 0x7fffffff || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
+    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
+    split(p);
+    if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    with_type(dtype, [&](auto e) {
+    with_type_and_width(dtype, U, [&](auto e, auto v) {
         using E = decltype(e);
+        constexpr int V = decltype(v)::value;
         if (p.chunks > 1)
-            chunk_kernel<E, false><<<(unsigned)(blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, nullptr, 0, 0);
-        scan_fwd_kernel<E><<<(unsigned)(blocks * p.chunks), kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
-                                                                             tile_states);
+            chunk_kernel<E, V, false><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, nullptr, 0, 0);
+        scan_fwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
+                                                                                  tile_states);
     });
     return swarm::record_hip_status();
 }
@@ -498,18 +548,19 @@ int32_t swarm_gated_scan_backward(int32_t dtype, int64_t n, int64_t T, int64_t U
     if (n == 0) return SWARM_OK;
     if (!gates || !tile_states || !d_gates || gates_t < 0 || gates_n < 0 || d_h_n < 0 || d_h_t < 0)
         return SWARM_ERR_ARG;
-    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, work};
-    int64_t blocks;
-    split(n, T, U, width_of(dtype), p.groups, blocks, p.chunk_tiles, p.chunks);
-    if (blocks * p.chunks > 0x7fffffff || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
+    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
+    split(p);
+    if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    with_type(dtype, [&](auto e) {
+    with_type_and_width(dtype, U, [&](auto e, auto v) {
         using E = decltype(e);
+        constexpr int V = decltype(v)::value;
         const E* dh = static_cast<const E*>(d_h);
+        const int64_t dt = dh ? d_h_t : gates_t;      // without d_h the loads go to the gates
         if (p.chunks > 1)
-            chunk_kernel<E, true><<<(unsigned)(blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, dh, d_h_n, d_h_t);
-        scan_bwd_kernel<E><<<(unsigned)(blocks * p.chunks), kThreads, 0, st>>>(p, tile_states, dh, d_h_n, d_h_t, d_last,
-                                                                             static_cast<E*>(d_gates), d_c0);
+            chunk_kernel<E, V, true><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, dh, d_h_n, dt);
+        scan_bwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, tile_states, dh, d_h_n, dt, d_last,
+                                                                                  static_cast<E*>(d_gates), d_c0);
     });
     return swarm::record_hip_status();
 }

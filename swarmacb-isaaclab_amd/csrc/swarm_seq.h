@@ -28,36 +28,43 @@ __device__ __forceinline__ float sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * -kLog2e));
 }
 
-// 16 bytes of elements at any address: global loads and stores of 16 bytes need no alignment on gfx950, so rows
-// of odd width and unaligned views take the same path. `valid` < V at the end of a row goes element by element.
-template <typename T>
+// N elements at any address, held as words (a 16-bit element in a register of its own would double what a tile
+// takes). Global loads and stores of up to 16 bytes need no alignment on gfx950, so rows of odd width and
+// unaligned views take the same path as aligned ones.
+template <typename T, int N = 16 / sizeof(T)>
 struct Pack {
-    static constexpr int V = 16 / sizeof(T);
-    T e[V];
+    static constexpr int kWords = (N * (int)sizeof(T) + 3) / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* __restrict__ p) {
+        w[kWords - 1] = 0u;
+        __builtin_memcpy(w, p, N * sizeof(T));
+    }
+    __device__ __forceinline__ void store(T* __restrict__ p) const { __builtin_memcpy(p, w, N * sizeof(T)); }
+
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            return __builtin_bit_cast(float, w[j]);
+        } else if constexpr (__is_same(T, bf16)) {
+            return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+        } else {
+            return (float)__builtin_bit_cast(f16, (uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu));
+        }
+    }
+    // rounds to nearest even
+    __device__ __forceinline__ void set(const float (&v)[N]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = __builtin_bit_cast(uint32_t, v[j]);
+        } else {
+            typedef float F2 __attribute__((ext_vector_type(2)));
+            typedef T T2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int j = 0; j < N; j += 2)
+                w[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{v[j], j + 1 < N ? v[j + 1 < N ? j + 1 : j] : 0.0f}), T2));
+        }
+    }
 };
-
-template <typename T>
-__device__ __forceinline__ Pack<T> load_pack(const T* __restrict__ p, int valid) {
-    Pack<T> r;
-    if (valid >= Pack<T>::V) {
-        __builtin_memcpy(&r, p, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < Pack<T>::V; ++j) r.e[j] = j < valid ? p[j] : (T)0.0f;
-    }
-    return r;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_pack(T* __restrict__ p, const Pack<T>& v, int valid) {
-    if (valid >= Pack<T>::V) {
-        __builtin_memcpy(p, &v, 16);
-    } else {
-#pragma unroll
-        for (int j = 0; j < Pack<T>::V; ++j)
-            if (j < valid) p[j] = v.e[j];
-    }
-}
 
 // Calls fn with a value of the element type that `dtype` names; false for an unknown dtype.
 template <typename F>
