@@ -2,42 +2,248 @@
 //
 //   s = x + r,  rstd = (mean(s^2) + eps)^-1/2,  n = s rstd,  y = n w
 //   d_x = d_r = rstd (w dy - n mean(w dy n)) + d_stream,   d_w = sum over rows of dy n
+//
+// Memory bound: a row is read once, held in registers by as many threads as it needs (a wave up to 2048 elements,
+// else a workgroup), and written once. Packs of 16 bytes at any alignment; the last pack of a row is moved left to
+// end with it, so no load crosses the row: the elements it shares with the pack before are left out of the sums and
+// not stored. The backward pass keeps every thread's columns over all rows of its workgroup and adds the weight
+// gradient there; the workgroups' sums are added in a fixed order by a second kernel.
+#include <type_traits>
+
 #include "swarm_seq.h"
 
 using namespace swarm_seq;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int64_t kSlabs = 512;   // row slabs of the weight gradient's partial sums
+constexpr int64_t kResident = 256 * 1024;   // threads of the backward pass, at most: four waves on each SIMD
+constexpr int kFinish = 1024;               // threads of the weight gradient's last sum
+constexpr int kFinishCols = 32;
 
-// the sum of v over the workgroup, in every thread
-__device__ __forceinline__ float block_sum(float v, float* red) {
+// One row's layout: GROUP threads (a wave, or the whole workgroup), EPT elements of each.
+template <typename T, int GROUP, int EPT>
+struct Row {
+    static constexpr int V = 16 / sizeof(T);
+    static constexpr int NP = EPT / V;
+    static constexpr int kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr int kRows = kThreads / GROUP;     // rows of a workgroup at a time
+    static constexpr int kWaves = kThreads / 64;
+
+    // pack i of a thread: its first column, and how many of its elements belong to the pack before
+    static __device__ __forceinline__ void place(int i, int lane, int64_t D, int64_t& start, int& skip) {
+        const int64_t want = (int64_t)(i * GROUP + lane) * V;
+        start = want < D - V ? want : D - V;
+        skip = want - start < V ? (int)(want - start) : V;
+    }
+};
+
+// Stores the elements of a pack that are its own.
+template <typename T, int N>
+__device__ __forceinline__ void store_own(T* p, const Pack<T, N>& v, int skip) {
+    if (skip == 0) {
+        v.store(p);
+    } else {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int k = 0; k < kWaves; ++k) s += red[k];
-    return s;
+        for (int j = 0; j < N; ++j)
+            if (j >= skip) p[j] = (T)v.get(j);
+    }
 }
 
+// the sum of v over a row's threads, in every one
+template <int GROUP>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if constexpr (GROUP > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < GROUP / 64; ++k) v += red[k];
+    }
+    return v;
+}
+
+template <typename T, int GROUP, int EPT>
+__global__ __launch_bounds__((Row<T, GROUP, EPT>::kThreads)) void norm_fwd_kernel(
+    int64_t rows, int64_t D, const T* __restrict__ x, int64_t xr, const T* __restrict__ res, int64_t rr,
+    const T* __restrict__ w, float eps, T* __restrict__ y, T* __restrict__ out, float* __restrict__ rstd) {
+    using R = Row<T, GROUP, EPT>;
+    __shared__ float red[R::kWaves];
+    const int lane = threadIdx.x % GROUP;
+    const int64_t row = (int64_t)blockIdx.x * R::kRows + threadIdx.x / GROUP;
+    if (row >= rows) return;      // whole rows: with GROUP > 64 a workgroup has one
+    Pack<T> a[R::NP], b[R::NP], wt[R::NP];
+#pragma unroll
+    for (int i = 0; i < R::NP; ++i) {
+        int64_t start;
+        int skip;
+        R::place(i, lane, D, start, skip);
+        a[i].load(x + row * xr + start);
+        if (res) b[i].load(res + row * rr + start);
+        if (w) wt[i].load(w + start);
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R::NP; ++i) {
+        int64_t start;
+        int skip;
+        R::place(i, lane, D, start, skip);
+        float own = 0.0f;
+#pragma unroll
+        for (int j = 0; j < R::V; ++j) {
+            const float s = a[i].get(j) + (res ? b[i].get(j) : 0.0f);
+            own += j >= skip ? s * s : 0.0f;
+        }
+        ss += own;
+    }
+    const float inv = 1.0f / sqrtf(row_sum<GROUP>(ss, red) / (float)D + eps);
+#pragma unroll
+    for (int i = 0; i < R::NP; ++i) {
+        int64_t start;
+        int skip;
+        R::place(i, lane, D, start, skip);
+        if (skip >= R::V) continue;
+        float s[R::V], n[R::V];
+#pragma unroll
+        for (int j = 0; j < R::V; ++j) {
+            s[j] = a[i].get(j) + (res ? b[i].get(j) : 0.0f);
+            n[j] = s[j] * inv * (w ? wt[i].get(j) : 1.0f);
+        }
+        Pack<T> v;
+        if (res) {
+            v.set(s);
+            store_own(out + row * D + start, v, skip);
+        }
+        v.set(n);
+        store_own(y + row * D + start, v, skip);
+    }
+    if (rstd && lane == 0) rstd[row] = inv;
+}
+
+template <typename T, int GROUP, int EPT>
+__global__ __launch_bounds__((Row<T, GROUP, EPT>::kThreads), 4) void norm_bwd_kernel(
+    int64_t rows, int64_t D, const T* __restrict__ s, int64_t sr, const T* __restrict__ w,
+    const float* __restrict__ rstd, const T* __restrict__ dy, int64_t dyr, const T* __restrict__ ds, int64_t dsr,
+    T* __restrict__ dx, float* __restrict__ partials) {
+    using R = Row<T, GROUP, EPT>;
+    __shared__ float red[R::kWaves];
+    extern __shared__ float sums[];     // [kRows][D]: the workgroup's weight gradient, where it has several rows
+    const int lane = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+    float dw[R::NP][R::V];
+#pragma unroll
+    for (int i = 0; i < R::NP; ++i)
+#pragma unroll
+        for (int j = 0; j < R::V; ++j) dw[i][j] = 0.0f;
+    // GROUP > 64: every thread of the workgroup has the same row, so the barriers of row_sum are reached by all
+    for (int64_t row = (int64_t)blockIdx.x * R::kRows + group; row < rows; row += (int64_t)gridDim.x * R::kRows) {
+        const float inv = rstd[row];
+        Pack<T> a[R::NP], g[R::NP], e[R::NP], wt[R::NP];
+#pragma unroll
+        for (int i = 0; i < R::NP; ++i) {
+            int64_t start;
+            int skip;
+            R::place(i, lane, D, start, skip);
+            a[i].load(s + row * sr + start);
+            g[i].load(dy + row * dyr + start);
+            if (ds) e[i].load(ds + row * dsr + start);
+            if (w) wt[i].load(w + start);
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R::NP; ++i) {
+            int64_t start;
+            int skip;
+            R::place(i, lane, D, start, skip);
+            float own = 0.0f;
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) {
+                const float t = g[i].get(j) * (a[i].get(j) * inv);
+                dw[i][j] += t;
+                own += j >= skip ? t * (w ? wt[i].get(j) : 1.0f) : 0.0f;
+            }
+            dot += own;
+        }
+        const float mean = row_sum<GROUP>(dot, red) / (float)D;
+#pragma unroll
+        for (int i = 0; i < R::NP; ++i) {
+            int64_t start;
+            int skip;
+            R::place(i, lane, D, start, skip);
+            if (skip >= R::V) continue;
+            float v[R::V];
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) {
+                v[j] = inv * (g[i].get(j) * (w ? wt[i].get(j) : 1.0f) - a[i].get(j) * inv * mean);
+                if (ds) v[j] += e[i].get(j);
+            }
+            Pack<T> out;
+            out.set(v);
+            store_own(dx + row * D + start, out, skip);
+        }
+    }
+    if (!partials) return;
+#pragma unroll
+    for (int i = 0; i < R::NP; ++i) {
+        int64_t start;
+        int skip;
+        R::place(i, lane, D, start, skip);
+        float* to = R::kRows > 1 ? sums + group * D + start : partials + blockIdx.x * D + start;
+#pragma unroll
+        for (int j = 0; j < R::V; ++j)
+            if (j >= skip) to[j] = dw[i][j];
+    }
+    if constexpr (R::kRows > 1) {
+        __syncthreads();
+        for (int64_t d = threadIdx.x; d < D; d += R::kThreads) {
+            float t = sums[d];
+#pragma unroll
+            for (int k = 1; k < R::kRows; ++k) t += sums[k * D + d];
+            partials[blockIdx.x * D + d] = t;
+        }
+    }
+}
+
+// d_w = column sums of the workgroups' partial sums, each column by kFinish / kFinishCols threads
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_fwd_kernel(int64_t rows, int64_t D, const T* __restrict__ x, int64_t xr,
-                                                            const T* __restrict__ res, int64_t rr,
-                                                            const T* __restrict__ w, float eps, T* __restrict__ y,
-                                                            T* __restrict__ out, float* __restrict__ rstd) {
-    __shared__ float red[kWaves];
+__global__ __launch_bounds__(kFinish) void weight_finish_kernel(int64_t count, int64_t D, const float* __restrict__ partials,
+                                                                T* __restrict__ dw) {
+    constexpr int kParts = kFinish / kFinishCols;
+    __shared__ float red[kParts][kFinishCols];
+    const int col = threadIdx.x % kFinishCols, part = threadIdx.x / kFinishCols;
+    const int64_t d = (int64_t)blockIdx.x * kFinishCols + col;
+    float acc = 0.0f;
+    if (d < D) {
+#pragma unroll 8
+        for (int64_t k = part; k < count; k += kParts) acc += partials[k * D + d];
+    }
+    red[part][col] = acc;
+    __syncthreads();
+    if (part != 0 || d >= D) return;
+#pragma unroll
+    for (int k = 1; k < kParts; ++k) acc += red[k][col];
+    dw[d] = (T)acc;
+}
+
+// Rows narrower than a pack or wider than a workgroup's registers: element by element, the row read again for the
+// second use.
+constexpr int kPlain = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kPlain) void plain_fwd_kernel(int64_t rows, int64_t D, const T* __restrict__ x, int64_t xr,
+                                                           const T* __restrict__ res, int64_t rr,
+                                                           const T* __restrict__ w, float eps, T* __restrict__ y,
+                                                           T* __restrict__ out, float* __restrict__ rstd) {
+    __shared__ float red[kPlain / 64];
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         float ss = 0.0f;
-        for (int64_t d = threadIdx.x; d < D; d += kThreads) {
+        for (int64_t d = threadIdx.x; d < D; d += kPlain) {
             const float s = (float)x[r * xr + d] + (res ? (float)res[r * rr + d] : 0.0f);
             ss += s * s;
         }
-        const float inv = 1.0f / sqrtf(block_sum(ss, red) / (float)D + eps);
-        for (int64_t d = threadIdx.x; d < D; d += kThreads) {
+        const float inv = 1.0f / sqrtf(row_sum<kPlain>(ss, red) / (float)D + eps);
+        for (int64_t d = threadIdx.x; d < D; d += kPlain) {
             const float s = (float)x[r * xr + d] + (res ? (float)res[r * rr + d] : 0.0f);
             if (res) out[r * D + d] = (T)s;
             y[r * D + d] = (T)(s * inv * (w ? (float)w[d] : 1.0f));
@@ -47,19 +253,19 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(int64_t rows, int64_
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_bwd_kernel(int64_t rows, int64_t D, const T* __restrict__ s, int64_t sr,
-                                                            const T* __restrict__ w, const float* __restrict__ rstd,
-                                                            const T* __restrict__ dy, int64_t dyr,
-                                                            const T* __restrict__ ds, int64_t dsr,
-                                                            T* __restrict__ dx) {
-    __shared__ float red[kWaves];
+__global__ __launch_bounds__(kPlain) void plain_bwd_kernel(int64_t rows, int64_t D, const T* __restrict__ s, int64_t sr,
+                                                           const T* __restrict__ w, const float* __restrict__ rstd,
+                                                           const T* __restrict__ dy, int64_t dyr,
+                                                           const T* __restrict__ ds, int64_t dsr,
+                                                           T* __restrict__ dx) {
+    __shared__ float red[kPlain / 64];
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const float inv = rstd[r];
         float dot = 0.0f;
-        for (int64_t d = threadIdx.x; d < D; d += kThreads)
+        for (int64_t d = threadIdx.x; d < D; d += kPlain)
             dot += (float)dy[r * dyr + d] * (w ? (float)w[d] : 1.0f) * ((float)s[r * sr + d] * inv);
-        const float mean = block_sum(dot, red) / (float)D;
-        for (int64_t d = threadIdx.x; d < D; d += kThreads) {
+        const float mean = row_sum<kPlain>(dot, red) / (float)D;
+        for (int64_t d = threadIdx.x; d < D; d += kPlain) {
             const float g = (float)dy[r * dyr + d] * (w ? (float)w[d] : 1.0f);
             float v = inv * (g - (float)s[r * sr + d] * inv * mean);
             if (ds) v += (float)ds[r * dsr + d];
@@ -70,12 +276,12 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(int64_t rows, int64_
 
 // partials[slab][d] = sum over the slab's rows of dy n
 template <typename T>
-__global__ __launch_bounds__(kThreads) void weight_partial_kernel(int64_t rows, int64_t D, int64_t slab,
-                                                                  const T* __restrict__ s, int64_t sr,
-                                                                  const float* __restrict__ rstd,
-                                                                  const T* __restrict__ dy, int64_t dyr,
-                                                                  float* __restrict__ partials) {
-    const int64_t d = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+__global__ __launch_bounds__(kPlain) void plain_weight_kernel(int64_t rows, int64_t D, int64_t slab,
+                                                              const T* __restrict__ s, int64_t sr,
+                                                              const float* __restrict__ rstd,
+                                                              const T* __restrict__ dy, int64_t dyr,
+                                                              float* __restrict__ partials) {
+    const int64_t d = (int64_t)blockIdx.x * kPlain + threadIdx.x;
     if (d >= D) return;
     const int64_t r0 = blockIdx.y * slab, r1 = r0 + slab < rows ? r0 + slab : rows;
     float acc = 0.0f;
@@ -83,21 +289,54 @@ __global__ __launch_bounds__(kThreads) void weight_partial_kernel(int64_t rows, 
     partials[blockIdx.y * D + d] = acc;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void weight_finish_kernel(int64_t slabs, int64_t D,
-                                                                 const float* __restrict__ partials,
-                                                                 T* __restrict__ dw) {
-    const int64_t d = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (d >= D) return;
-    float acc = 0.0f;
-    for (int64_t k = 0; k < slabs; ++k) acc += partials[k * D + d];
-    dw[d] = (T)acc;
+// Threads and elements a row takes. Forward: few threads with many loads each, so that rows up to 2048 need no
+// barrier. Backward: 8 elements a thread, since a thread also holds the weight and its sums of them; with 16 the
+// kernel took 135 registers, three waves a SIMD, and 123 us where it now takes FIXME (16384 x 4096, bf16).
+struct Plan {
+    int group, ept;      // 0: the plain kernels
+};
+
+Plan plan_of(int64_t D, int64_t V, bool backward) {
+    if (D < V || D > 16384) return {0, 0};
+    if (D <= 512) return {64, 8};
+    if (D <= 1024) return backward ? Plan{128, 8} : Plan{64, 16};
+    if (D <= 2048) return backward ? Plan{256, 8} : Plan{64, 32};
+    if (D <= 4096) return backward ? Plan{512, 8} : Plan{256, 16};
+    if (D <= 8192) return backward ? Plan{1024, 8} : Plan{512, 16};
+    return {1024, 16};
 }
 
-void slabs_of(int64_t rows, int64_t& slab, int64_t& slabs) {
-    slab = (rows + kSlabs - 1) / kSlabs;
-    slabs = slab ? (rows + slab - 1) / slab : 0;
+template <bool BACKWARD, typename F>
+void with_plan(const Plan& p, F&& fn) {
+    using std::integral_constant;
+    auto call = [&](auto g, auto n) {
+        if (p.group == g && p.ept == n) fn(g, n);
+    };
+    call(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+    call(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+    if constexpr (BACKWARD) {
+        call(integral_constant<int, 128>{}, integral_constant<int, 8>{});
+        call(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+        call(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+        call(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+    } else {
+        call(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+        call(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+        call(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+        call(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+    }
 }
+
+int64_t at_a_time(const Plan& p) { return p.group == 64 ? 4 : 1; }
+
+// Partial sums of the weight gradient: one for each workgroup of the backward pass.
+int64_t partials_of(int64_t rows, const Plan& p) {
+    const int64_t per = at_a_time(p), blocks = (rows + per - 1) / per;
+    const int64_t most = kResident / (p.group <= 64 ? 256 : p.group);
+    return blocks < most ? blocks : most;
+}
+
+bool fits_grid(int64_t blocks) { return blocks <= 0x7fffffff; }
 
 }  // namespace
 
@@ -105,9 +344,12 @@ extern "C" {
 
 int64_t swarm_residual_norm_workspace(int64_t rows, int64_t D) {
     if (rows < 0 || D < 1 || !sane(rows, D)) return SWARM_ERR_ARG;
-    int64_t slab, slabs;
-    slabs_of(rows, slab, slabs);
-    return slabs * D;
+    int64_t most = 0;
+    for (int64_t V : {4, 8}) {
+        const int64_t n = partials_of(rows, plan_of(D, V, true));
+        if (n > most) most = n;
+    }
+    return most * D;
 }
 
 int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, const void* x, int64_t x_row,
@@ -115,13 +357,25 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
                                     void* stream_out, float* rstd, void* stream) {
     if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D) || !(eps >= 0.0f)) return SWARM_ERR_ARG;
     if (rows == 0) return SWARM_OK;
-    if (!x || !y || (residual && !stream_out) || x_row < 0 || res_row < 0) return SWARM_ERR_ARG;
-    const unsigned blocks = (unsigned)(rows < 65536 ? rows : 65536);
+    const Plan plan = plan_of(D, dtype == SWARM_F32 ? 4 : 8, false);
+    const int64_t blocks = (rows + at_a_time(plan) - 1) / at_a_time(plan);
+    if (!x || !y || (residual && !stream_out) || x_row < 0 || res_row < 0 || !fits_grid(blocks)) return SWARM_ERR_ARG;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        norm_fwd_kernel<E><<<blocks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            rows, D, static_cast<const E*>(x), x_row, static_cast<const E*>(residual), res_row,
-            static_cast<const E*>(weight), eps, static_cast<E*>(y), static_cast<E*>(stream_out), rstd);
+        const E *xp = static_cast<const E*>(x), *rp = static_cast<const E*>(residual);
+        const E* wp = static_cast<const E*>(weight);
+        E *yp = static_cast<E*>(y), *op = static_cast<E*>(stream_out);
+        if (plan.group == 0) {
+            plain_fwd_kernel<E><<<(unsigned)(rows < 65536 ? rows : 65536), kPlain, 0, st>>>(rows, D, xp, x_row, rp, res_row,
+                                                                                        wp, eps, yp, op, rstd);
+            return;
+        }
+        with_plan<false>(plan, [&](auto g, auto n) {
+            constexpr int G = decltype(g)::value, N = decltype(n)::value;
+            norm_fwd_kernel<E, G, N><<<(unsigned)blocks, Row<E, G, N>::kThreads, 0, st>>>(rows, D, xp, x_row, rp, res_row,
+                                                                                        wp, eps, yp, op, rstd);
+        });
     });
     return swarm::record_hip_status();
 }
@@ -130,26 +384,39 @@ int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, con
                                      const void* weight, const float* rstd, const void* d_y, int64_t dy_row,
                                      const void* d_stream, int64_t ds_row, void* d_x, void* d_weight, float* work,
                                      void* stream) {
-    if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D) || D > 0x7fffffffLL * kThreads) return SWARM_ERR_ARG;
-    if (d_weight && rows > 0 && !work) return SWARM_ERR_ARG;
+    if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D)) return SWARM_ERR_ARG;
+    const int64_t cols = (D + kFinishCols - 1) / kFinishCols;
+    if ((d_weight && rows > 0 && !work) || !fits_grid(cols)) return SWARM_ERR_ARG;
     if (rows == 0 && !d_weight) return SWARM_OK;
     if (rows > 0 && (!sum || !rstd || !d_y || !d_x || sum_row < 0 || dy_row < 0 || ds_row < 0)) return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned blocks = (unsigned)(rows < 65536 ? rows : 65536);
-    const unsigned cols = (unsigned)((D + kThreads - 1) / kThreads);
-    int64_t slab, slabs;
-    slabs_of(rows, slab, slabs);
+    const Plan plan = plan_of(D, dtype == SWARM_F32 ? 4 : 8, true);
+    int64_t count = partials_of(rows, plan);
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        if (rows > 0)
-            norm_bwd_kernel<E><<<blocks, kThreads, 0, st>>>(
-                rows, D, static_cast<const E*>(sum), sum_row, static_cast<const E*>(weight), rstd,
-                static_cast<const E*>(d_y), dy_row, static_cast<const E*>(d_stream), ds_row, static_cast<E*>(d_x));
-        if (!d_weight) return;
-        if (rows > 0)
-            weight_partial_kernel<E><<<dim3(cols, (unsigned)slabs), kThreads, 0, st>>>(
-                rows, D, slab, static_cast<const E*>(sum), sum_row, rstd, static_cast<const E*>(d_y), dy_row, work);
-        weight_finish_kernel<E><<<cols, kThreads, 0, st>>>(slabs, D, work, static_cast<E*>(d_weight));
+        const E *sp = static_cast<const E*>(sum), *wp = static_cast<const E*>(weight);
+        const E *yp = static_cast<const E*>(d_y), *dp = static_cast<const E*>(d_stream);
+        E* xp = static_cast<E*>(d_x);
+        float* partials = d_weight ? work : nullptr;
+        if (rows > 0 && plan.group == 0) {
+            plain_bwd_kernel<E><<<(unsigned)(rows < 65536 ? rows : 65536), kPlain, 0, st>>>(rows, D, sp, sum_row, wp, rstd,
+                                                                                        yp, dy_row, dp, ds_row, xp);
+            const int64_t slab = (rows + count - 1) / count;
+            count = (rows + slab - 1) / slab;
+            if (d_weight)
+                plain_weight_kernel<E><<<dim3((unsigned)((D + kPlain - 1) / kPlain), (unsigned)count), kPlain, 0, st>>>(
+                    rows, D, slab, sp, sum_row, rstd, yp, dy_row, work);
+        } else if (rows > 0) {
+            with_plan<true>(plan, [&](auto g, auto n) {
+                constexpr int G = decltype(g)::value, N = decltype(n)::value;
+                using R = Row<E, G, N>;
+                const size_t lds = partials && R::kRows > 1 ? R::kRows * (size_t)D * sizeof(float) : 0;
+                norm_bwd_kernel<E, G, N><<<(unsigned)count, R::kThreads, lds, st>>>(rows, D, sp, sum_row, wp, rstd, yp,
+                                                                                  dy_row, dp, ds_row, xp, partials);
+            });
+        }
+        if (d_weight)
+            weight_finish_kernel<E><<<(unsigned)cols, kFinish, 0, st>>>(count, D, work, static_cast<E*>(d_weight));
     });
     return swarm::record_hip_status();
 }
