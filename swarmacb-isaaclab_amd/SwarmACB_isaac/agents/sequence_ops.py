@@ -36,8 +36,25 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(t: torch.Tensor):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _stream(t: torch.Tensor) -> int:
+    """The current stream of t's device, without building a torch.cuda.Stream (2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _once(backward):
+    """once_differentiable for a backward whose gradients are new tensors. Its wrapper costs 9 us a call and is
+    only needed where a graph of the gradients is asked for, which is when gradients are recorded in here."""
+    wrapped = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+def _flat(t: torch.Tensor, n: int) -> torch.Tensor:
+    """t as n contiguous values."""
+    return (t if t.dim() == 1 else t.reshape(n)).contiguous()
 
 
 def _check(rc: int, what: str):
@@ -96,32 +113,37 @@ def _no_grad_operand(t, what: str):
 
 # -------------------------------------------------------------------------------- gated recurrence
 
+def _scan_forward(gates, state, keep, lengths, save: bool):
+    """(h, last state, tile states or None)"""
+    n, T, U3 = gates.shape
+    U = U3 // 3
+    lib = _native.load()
+    with _on(gates):
+        h = torch.empty(n, T, U, dtype=gates.dtype, device=gates.device)
+        last = torch.empty(n, U, dtype=torch.float32, device=gates.device)
+        tiles = (torch.empty(n, _native.gated_tiles(T), U, dtype=torch.float32, device=gates.device)
+                 if save else None)
+        work = _scan_work(lib, n, T, U, gates.device)
+        _check(lib.swarm_gated_scan_forward(_DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1),
+                                            _p(state), _p(keep), _p(lengths), _p(h), _p(last), _p(tiles), _p(work),
+                                            _stream(gates)), "swarm_gated_scan_forward")
+    return h, last, tiles
+
+
 class _GatedScan(torch.autograd.Function):
     """swarm_gated_scan_forward / _backward. The backward forms the states again from one saved state per
     tile of steps, so nothing of the size of the sequence is kept but the inputs."""
 
     @staticmethod
-    def forward(ctx, gates, state, keep, lengths, save: bool):
-        n, T, U3 = gates.shape
-        U = U3 // 3
-        dt = _DTYPES[gates.dtype]
-        lib = _native.load()
-        with _on(gates):
-            h = torch.empty(n, T, U, dtype=gates.dtype, device=gates.device)
-            last = torch.empty(n, U, dtype=torch.float32, device=gates.device)
-            tiles = (torch.empty(n, _native.gated_tiles(T), U, dtype=torch.float32, device=gates.device)
-                     if save else None)
-            work = _scan_work(lib, n, T, U, gates.device)
-            _check(lib.swarm_gated_scan_forward(dt, n, T, U, _p(gates), gates.stride(0), gates.stride(1), _p(state),
-                                                _p(keep), _p(lengths), _p(h), _p(last), _p(tiles), _p(work),
-                                                _stream(gates)), "swarm_gated_scan_forward")
+    def forward(ctx, gates, state, keep, lengths):
+        h, last, tiles = _scan_forward(gates, state, keep, lengths, True)
         ctx.save_for_backward(gates, keep, lengths, tiles)
         ctx.has_state = state is not None
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_h, d_last):
         gates, keep, lengths, tiles = ctx.saved_tensors
         n, T, U3 = gates.shape
@@ -140,7 +162,7 @@ class _GatedScan(torch.autograd.Function):
                 _DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1), _p(keep), _p(lengths),
                 _p(tiles), _p(d_h), d_h.stride(0) if d_h is not None else 0, d_h.stride(1) if d_h is not None else 0,
                 _p(d_last), _p(d_gates), _p(d_state), _p(work), _stream(gates)), "swarm_gated_scan_backward")
-        return d_gates, d_state, None, None, None
+        return d_gates, d_state, None, None
 
 
 def _scan_work(lib, n: int, T: int, U: int, device):
@@ -185,8 +207,10 @@ def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, kee
         lengths = lengths.to(torch.int64).contiguous()
     if state is not None:
         state = state.contiguous()
-    save = torch.is_grad_enabled() and (gates.requires_grad or (state is not None and state.requires_grad))
-    return _GatedScan.apply(_rows(gates), state, keep, lengths, save)
+    gates = _rows(gates)
+    if torch.is_grad_enabled() and (gates.requires_grad or (state is not None and state.requires_grad)):
+        return _GatedScan.apply(gates, state, keep, lengths)
+    return _scan_forward(gates, state, keep, lengths, False)[:2]
 
 
 def _plain_scan(gates, state, keep, lengths):
@@ -251,27 +275,33 @@ def gated_recurrence_step(gates: torch.Tensor, state: torch.Tensor, keep: torch.
 
 # ------------------------------------------------------------------------------- residual RMS norm
 
+def _norm_forward(x, residual, weight, eps: float, save: bool):
+    """(y, stream or None, rstd or None)"""
+    rows, D = x.shape
+    with _on(x):
+        y = torch.empty(rows, D, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(y) if residual is not None else None
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save else None
+        _check(_native.load().swarm_residual_norm_forward(
+            _DTYPES[x.dtype], rows, D, _p(x), x.stride(0), _p(residual),
+            residual.stride(0) if residual is not None else 0, _p(weight), eps, _p(y), _p(out), _p(rstd),
+            _stream(x)), "swarm_residual_norm_forward")
+    return y, out, rstd
+
+
 class _ResidualNorm(torch.autograd.Function):
     """swarm_residual_norm_forward / _backward over (rows, D); the saved sum is the stream itself."""
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps: float):
-        rows, D = x.shape
-        with _on(x):
-            y = torch.empty(rows, D, dtype=x.dtype, device=x.device)
-            out = torch.empty_like(y) if residual is not None else None
-            rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-            _check(_native.load().swarm_residual_norm_forward(
-                _DTYPES[x.dtype], rows, D, _p(x), x.stride(0), _p(residual),
-                residual.stride(0) if residual is not None else 0, _p(weight), eps, _p(y), _p(out), _p(rstd),
-                _stream(x)), "swarm_residual_norm_forward")
+        y, out, rstd = _norm_forward(x, residual, weight, eps, True)
         ctx.save_for_backward(out if out is not None else x, weight, rstd)
         ctx.two = residual is not None
         ctx.set_materialize_grads(False)
         return (y, out) if out is not None else y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, d_y, d_out=None):
         s, weight, rstd = ctx.saved_tensors
         rows, D = s.shape
@@ -315,12 +345,19 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
         return y.to(x.dtype), (x if residual is None else s.to(x.dtype))
     D = x.shape[-1]
     rows = x.numel() // D
-    x2 = _rows(x.reshape(rows, D))
-    r2 = None if residual is None else _rows(residual.reshape(rows, D))
-    out = _ResidualNorm.apply(x2, r2, None if weight is None else weight.contiguous(), float(eps))
+    flat = x.dim() == 2
+    x2 = _rows(x if flat else x.reshape(rows, D))
+    r2 = None if residual is None else _rows(residual if flat else residual.reshape(rows, D))
+    w = None if weight is None else weight.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or (r2 is not None and r2.requires_grad)
+                                    or (w is not None and w.requires_grad)):
+        out = _ResidualNorm.apply(x2, r2, w, float(eps))
+        y, stream = (out, None) if residual is None else out
+    else:
+        y, stream, _ = _norm_forward(x2, r2, w, float(eps), False)
     if residual is None:
-        return out.view(x.shape), x
-    return out[0].view(x.shape), out[1].view(x.shape)
+        return (y if flat else y.view(x.shape)), x
+    return (y, stream) if flat else (y.view(x.shape), stream.view(x.shape))
 
 
 # ------------------------------------------------------------------------------------- policy loss
@@ -348,7 +385,7 @@ class _PolicyLossFromLogits(torch.autograd.Function):
         return loss, terms
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g, _terms):
         logits, actions, stats, used = ctx.saved_tensors
         M, K = logits.shape
@@ -370,7 +407,7 @@ def _logit_rows(logits, actions, what: str):
         raise ValueError(f"{what}: actions are needed")
     K = logits.shape[-1]
     M = logits.numel() // K
-    return _rows(logits.reshape(M, K)), actions.reshape(M).to(torch.int64).contiguous(), M, K
+    return _rows(logits if logits.dim() == 2 else logits.reshape(M, K)), _flat(actions.to(torch.int64), M), M, K
 
 
 def categorical_log_probs(logits: torch.Tensor, actions: torch.Tensor):
@@ -435,9 +472,9 @@ def categorical_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_log
         raise ValueError(f"{what}: clip {clip} leaves no interval")
     if kl_coef != 0.0 and ref_log_probs is None:
         raise ValueError(f"{what}: kl_coef needs ref_log_probs")
-    old, adv = old_log_probs.reshape(M).contiguous(), advantages.reshape(M).contiguous()
-    ref = None if ref_log_probs is None else ref_log_probs.reshape(M).contiguous()
-    active = None if mask is None else mask.reshape(M).contiguous()
+    old, adv = _flat(old_log_probs, M), _flat(advantages, M)
+    ref = None if ref_log_probs is None else _flat(ref_log_probs, M)
+    active = None if mask is None else _flat(mask, M)
     d = None if denom is None else denom.reshape(()).contiguous()
     if not z.is_cuda:
         return _plain_policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef))
