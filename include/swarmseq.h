@@ -94,7 +94,8 @@ int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits,
  *     terms[4] = the means of pg, kl, H and of the share of rows with r outside [clip_lo, clip_hi]
  * l - old and d are bounded to [-20, 20] (no gradient outside). denom: *denom if given, else
  * max(active rows, 1); the one used goes to *used_denom. Inactive rows are not looked at.
- *   old, ref, adv: [M] f32; row_stats: [M][4] f32 for the backward pass; partials:
+ *   old, ref, adv: [M] f32; row_stats: [M][4] f32 for the backward pass; d_logits: [M][K], the gradient for an
+ *   incoming gradient of 1, formed from the logits while they are at hand (NULL: not formed); partials:
  *   SWARM_POLICY_LOSS_PARTIALS floats of workspace. An active row's action outside [0, K) makes the loss NaN
  *   and sets *bad_actions to 1. */
 #define SWARM_POLICY_LOSS_PARTIALS (2048 * 6)
@@ -102,12 +103,14 @@ int32_t swarm_policy_loss_forward(int32_t dtype, int64_t M, int64_t K, const voi
                                   const int64_t* actions, const float* old_log_probs, const float* ref_log_probs,
                                   const float* advantages, const uint8_t* mask_u8, const float* denom, float clip_lo,
                                   float clip_hi, float kl_coef, float entropy_coef, float* loss, float* terms,
-                                  float* used_denom, float* row_stats, float* partials, int32_t* bad_actions,
-                                  void* stream);
-/* d_logits: [M][K], every element (zeros on inactive rows), for the incoming gradient *grad of *loss. */
+                                  float* used_denom, float* row_stats, void* d_logits, float* partials,
+                                  int32_t* bad_actions, void* stream);
+/* d_logits: [M][K], every element (zeros on inactive rows), for the incoming gradient *grad of *loss. have_unit:
+ * d_logits holds what the forward call put there, and stays as it is where *grad is 1. */
 int32_t swarm_policy_loss_backward(int32_t dtype, int64_t M, int64_t K, const void* logits, int64_t row_stride,
                                    const int64_t* actions, float entropy_coef, const float* row_stats,
-                                   const float* used_denom, const float* grad, void* d_logits, void* stream);
+                                   const float* used_denom, const float* grad, int32_t have_unit, void* d_logits,
+                                   void* stream);
 
 #ifdef __cplusplus
 }

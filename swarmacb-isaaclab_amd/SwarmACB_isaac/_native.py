@@ -285,9 +285,9 @@ def load() -> C.CDLL:
     lib.swarm_log_probs.restype = i32
     lib.swarm_log_probs.argtypes = [i32, i64, i64, vp, i64] + [vp] * 5
     lib.swarm_policy_loss_forward.restype = i32
-    lib.swarm_policy_loss_forward.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6 + [f32] * 4 + [vp] * 7
+    lib.swarm_policy_loss_forward.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6 + [f32] * 4 + [vp] * 8
     lib.swarm_policy_loss_backward.restype = i32
-    lib.swarm_policy_loss_backward.argtypes = [i32, i64, i64, vp, i64, vp, f32] + [vp] * 5
+    lib.swarm_policy_loss_backward.argtypes = [i32, i64, i64, vp, i64, vp, f32, vp, vp, vp, i32, vp, vp]
     if lib.swarm_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libswarmstep ABI {lib.swarm_abi_version()} != expected {ABI_VERSION}")
     _lib = lib

@@ -362,24 +362,34 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
 
 # ------------------------------------------------------------------------------------- policy loss
 
+def _loss_forward(logits, actions, old, adv, ref, mask_u, denom, lo, hi, kl_coef, entropy_coef, save: bool):
+    """(loss, terms, row statistics, denominator, gradient for an incoming gradient of 1 or None)"""
+    M, K = logits.shape
+    dev = logits.device
+    with _on(logits):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        terms = torch.empty(4, dtype=torch.float32, device=dev)
+        used = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(_native.POLICY_LOSS_PARTIALS + 4 * M, dtype=torch.float32, device=dev)
+        unit = torch.empty(M, K, dtype=logits.dtype, device=dev) if save and logits.dtype != torch.float16 else None
+        stats = work.data_ptr() + 4 * _native.POLICY_LOSS_PARTIALS
+        _check(_native.load().swarm_policy_loss_forward(
+            _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), _p(old), _p(ref), _p(adv),
+            _p(mask_u), _p(denom), lo, hi, kl_coef, entropy_coef, _p(loss), _p(terms), _p(used), stats, _p(unit),
+            _p(work), _p(_bad_action_flag(dev)), _stream(logits)), "swarm_policy_loss_forward")
+    return loss, terms, work, used, unit
+
+
 class _PolicyLossFromLogits(torch.autograd.Function):
-    """swarm_policy_loss_forward / _backward."""
+    """swarm_policy_loss_forward / _backward. The forward call, which has the logits at hand, forms the gradient
+    for an incoming gradient of 1 as well (not in float16, where losses are scaled); the first backward call
+    hands it out, written anew if the incoming gradient is another one, and later calls form their own."""
 
     @staticmethod
     def forward(ctx, logits, actions, old, adv, ref, mask_u, denom, lo, hi, kl_coef, entropy_coef):
-        M, K = logits.shape
-        dev = logits.device
-        with _on(logits):
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            terms = torch.empty(4, dtype=torch.float32, device=dev)
-            used = torch.empty((), dtype=torch.float32, device=dev)
-            stats = torch.empty(M, 4, dtype=torch.float32, device=dev)
-            partials = torch.empty(_native.POLICY_LOSS_PARTIALS, dtype=torch.float32, device=dev)
-            _check(_native.load().swarm_policy_loss_forward(
-                _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), _p(old), _p(ref), _p(adv),
-                _p(mask_u), _p(denom), lo, hi, kl_coef, entropy_coef, _p(loss), _p(terms), _p(used),
-                _p(stats), _p(partials), _p(_bad_action_flag(dev)), _stream(logits)), "swarm_policy_loss_forward")
-        ctx.save_for_backward(logits, actions, stats, used)
+        loss, terms, work, used, ctx.unit = _loss_forward(logits, actions, old, adv, ref, mask_u, denom, lo, hi,
+                                                          kl_coef, entropy_coef, True)
+        ctx.save_for_backward(logits, actions, work, used)
         ctx.entropy_coef = entropy_coef
         ctx.mark_non_differentiable(terms)
         return loss, terms
@@ -387,14 +397,18 @@ class _PolicyLossFromLogits(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, g, _terms):
-        logits, actions, stats, used = ctx.saved_tensors
+        logits, actions, work, used = ctx.saved_tensors
         M, K = logits.shape
+        d, ctx.unit = ctx.unit, None
         with _on(logits):
-            d = torch.empty(M, K, dtype=logits.dtype, device=logits.device)
+            have = d is not None
+            if not have:
+                d = torch.empty(M, K, dtype=logits.dtype, device=logits.device)
             g = g.contiguous()
             _check(_native.load().swarm_policy_loss_backward(
-                _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), ctx.entropy_coef, _p(stats),
-                _p(used), _p(g), _p(d), _stream(logits)), "swarm_policy_loss_backward")
+                _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), ctx.entropy_coef,
+                work.data_ptr() + 4 * _native.POLICY_LOSS_PARTIALS, _p(used), _p(g), have, _p(d), _stream(logits)),
+                "swarm_policy_loss_backward")
         return (d,) + (None,) * 10
 
 
@@ -478,8 +492,11 @@ def categorical_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_log
     d = None if denom is None else denom.reshape(()).contiguous()
     if not z.is_cuda:
         return _plain_policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef))
-    return _PolicyLossFromLogits.apply(z, a, old, adv, ref, None if active is None else active.view(torch.uint8), d,
-                                       lo, hi, float(kl_coef), float(entropy_coef))
+    args = (z, a, old, adv, ref, None if active is None else active.view(torch.uint8), d, lo, hi, float(kl_coef),
+            float(entropy_coef))
+    if torch.is_grad_enabled() and z.requires_grad:
+        return _PolicyLossFromLogits.apply(*args)
+    return _loss_forward(*args, False)[:2]
 
 
 def _plain_policy_loss(z, a, old, adv, ref, active, denom, lo, hi, kl_coef, entropy_coef):

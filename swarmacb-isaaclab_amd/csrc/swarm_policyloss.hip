@@ -1,93 +1,297 @@
 // swarm_policyloss.hip — log-probabilities and the clipped policy loss with a KL term, from logits
 // (include/swarmseq.h: swarm_log_probs, swarm_policy_loss_*).
 //
-// Per row of K logits z with the taken action a, m = max z, s = sum exp(z - m), t = sum exp(z - m) (z - m):
-//   L = m + log s,  l = z_a - L,  H = log s - t / s,  p_k = exp(z_k - L)
-//   dz_k = (1 / denom) [ g (1[k = a] - p_k) + entropy_coef p_k (log p_k + H) ],
+// Per row of K logits z with the taken action a, m = max z, d_k = z_k - m, s = sum exp d_k, t = sum exp(d_k) d_k:
+//   log p_k = d_k - log s,  l = log p_a,  H = log s - t / s
+//   dz_k = c [ g (1[k = a] - p_k) + entropy_coef p_k (log p_k + H) ],   c = incoming gradient / denominator,
 //   g = d pg / d l + kl_coef (1 - exp(ref - l)).
-// m, s and t are gathered in one pass: a running maximum rescales the two sums when it grows. A logit of -inf
-// adds nothing to either sum and has no gradient.
+// A logit of -inf adds nothing to either sum and has no gradient: its exp is 0, and so are the products it enters.
+//
+// Memory bound. A row is read once and held in registers by as many threads as it needs; maximum, then both sums,
+// are reduced over them. Since the denominator does not depend on the logits, the gradient for an incoming gradient
+// of 1 follows at once, from the same registers: reading the logits once and writing their gradient is all the
+// traffic there is. The backward call keeps that gradient if the incoming one is 1, and otherwise forms it again
+// (scaling a rounded gradient would round it twice). Rows that no workgroup holds are read twice.
+#include <type_traits>
+
 #include "swarm_seq.h"
 
 using namespace swarm_seq;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kMaxBlocks = 2048;      // SWARM_POLICY_LOSS_PARTIALS = 6 sums for each
+constexpr int kMaxBlocks = 2048;      // SWARM_POLICY_LOSS_PARTIALS = kSums for each
 constexpr int kSums = 6;              // pg, kl, H, outside, pg + kl_coef kl - entropy_coef H, active rows
 constexpr float kBound = 20.0f;       // bound of the log-ratios
-
-struct Stats {
-    float m, s, t;
-};
+constexpr float kInactive = -1.0f;    // log s of a row that takes no part (log s >= 0 elsewhere: exp d = 1 at the maximum)
+constexpr int64_t kCountHere = 8192;  // masks up to this many rows are counted by every workgroup itself
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-__device__ __forceinline__ void add_logit(Stats& a, float z) {
-    if (z > a.m) {
-        const float d = a.m - z;
-        if (a.m != -INFINITY) {
-            const float e = exp_of(d);
-            a.t = e * (a.t + d * a.s);
-            a.s *= e;
-        }
-        a.m = z;
-    }
-    if (z != -INFINITY) {
-        const float d = z - a.m, e = exp_of(d);
-        a.s += e;
-        a.t += e > 0.0f ? e * d : e;   // e * d: 0 * -inf for a logit far below; a NaN stays
-    }
-}
-
-__device__ __forceinline__ Stats merge(const Stats& a, const Stats& b) {
-    if (b.m == -INFINITY && b.s == 0.0f) return a;
-    if (a.m == -INFINITY && a.s == 0.0f) return b;
-    Stats r;
-    r.m = fmaxf(a.m, b.m);
-    const float da = a.m - r.m, db = b.m - r.m, ea = exp_of(da), eb = exp_of(db);
-    r.s = ea * a.s + eb * b.s;
-    r.t = (ea > 0.0f || ea != ea ? ea * (a.t + da * a.s) : 0.0f) + (eb > 0.0f || eb != eb ? eb * (b.t + db * b.s) : 0.0f);
-    return r;
-}
-
-template <typename T>
-__device__ Stats row_stats_of(const T* __restrict__ z, int64_t K, Stats* red) {
-    Stats a{-INFINITY, 0.0f, 0.0f};
-    for (int64_t k = threadIdx.x; k < K; k += kThreads) add_logit(a, (float)z[k]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        Stats b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
-        a = merge(a, b);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = red[0];
-    for (int k = 1; k < kWaves; ++k) a = merge(a, red[k]);
-    return a;
-}
+// An exponent as a factor: finite, so that 0 = exp(-inf) times it is 0. (A NaN is dropped here; its exp is the NaN.)
+__device__ __forceinline__ float finite(float d) { return fmaxf(d, -1e30f); }
 
 // clamp that keeps a NaN
 __device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return x < lo ? lo : (x > hi ? hi : x); }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void log_probs_kernel(int64_t M, int64_t K, const T* __restrict__ logits, int64_t ld,
-                                                             const int64_t* __restrict__ actions,
-                                                             float* __restrict__ logp, float* __restrict__ ent,
-                                                             int32_t* __restrict__ bad) {
-    __shared__ Stats red[kWaves];
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        const T* z = logits + m * ld;
-        const Stats a = row_stats_of(z, K, red);
-        if (threadIdx.x == 0) {
-            const int64_t k = actions[m];
-            const bool in = k >= 0 && k < K;
-            const float ls = logf(a.s);
-            logp[m] = in ? ((float)z[k] - a.m) - ls : NAN;
-            ent[m] = ls - a.t / a.s;
+// Reductions over a row's GROUP threads, in every one.
+template <int GROUP>
+__device__ __forceinline__ float group_max(float v, float* red) {
+#pragma unroll
+    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    if constexpr (GROUP > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int k = 1; k < GROUP / 64; ++k) v = fmaxf(v, red[k]);
+    }
+    return v;
+}
+
+template <int GROUP>
+__device__ __forceinline__ void group_sums(float& s, float& t, float* red) {
+#pragma unroll
+    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o);
+        t += __shfl_xor(t, o);
+    }
+    if constexpr (GROUP > 64) {
+        constexpr int W = GROUP / 64;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s, red[W + (threadIdx.x >> 6)] = t;
+        __syncthreads();
+        s = t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) s += red[k], t += red[W + k];
+    }
+}
+
+// A row of few logits: E of them in each of LPR lanes, lane after lane.
+template <typename E, int LPR, int N>
+struct Narrow {
+    using T = E;
+    static constexpr int kGroup = LPR, kThreads = 256;
+    static constexpr bool kHeld = true;
+    float z[N];
+
+    __device__ __forceinline__ void load(const T* p, int lane, int64_t K) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = lane + i * LPR;
+            z[i] = (float)p[k < (int)K ? k : (int)K - 1];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = lane + i * LPR < (int)K ? z[i] : -INFINITY;
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f(z[i]);
+    }
+    // out[k] = f(z_k), and more at the action
+    template <typename F>
+    __device__ __forceinline__ void write(T* out, int lane, int64_t K, int64_t a, float more, F&& f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = lane + i * LPR;
+            if (k < (int)K) out[k] = (T)(f(z[i]) + (k == a ? more : 0.0f));
+        }
+    }
+};
+
+// Pack i of a thread of a long row: its first column, and how many of its elements belong to the pack before (the
+// last pack is moved left to end with the row).
+template <int V>
+__device__ __forceinline__ void place(int64_t pack, int64_t K, int64_t& start, int& skip) {
+    const int64_t want = pack * V;
+    start = want < K - V ? want : K - V;
+    skip = want - start < V ? (int)(want - start) : V;
+}
+
+// Stores f of a pack's own elements, and more at the action.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void write_pack(T* out, const Pack<T>& x, int64_t start, int skip, int64_t a, float more,
+                                           F&& f) {
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = f(x.get(j));
+    const uint64_t at = (uint64_t)(a - start);
+    if (at < (uint64_t)V) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += at == (uint64_t)j ? more : 0.0f;
+    }
+    Pack<T> w;
+    w.set(v);
+    if (skip == 0) {
+        w.store(out + start);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j >= skip) out[start + j] = (T)w.get(j);
+    }
+}
+
+// A longer row: EPT logits of each of GROUP threads, in packs of 16 bytes at any alignment.
+template <typename E, int GROUP, int EPT>
+struct Wide {
+    using T = E;
+    static constexpr int kGroup = GROUP, kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr bool kHeld = true;
+    static constexpr int V = 16 / sizeof(T), NP = EPT / V;
+    Pack<T> x[NP];
+    int used;      // packs of a thread that any thread needs
+
+    // as place(), in 32 bits: one register an address, next to the row's uniform base
+    static __device__ __forceinline__ void at(int i, int lane, int64_t K, uint32_t& start, int& skip) {
+        const uint32_t want = (uint32_t)(i * GROUP + lane) * V, last = (uint32_t)K - V;
+        start = want < last ? want : last;
+        skip = want - start < (uint32_t)V ? (int)(want - start) : V;
+    }
+
+    __device__ __forceinline__ void load(const T* p, int lane, int64_t K) {
+        used = (int)((K + GROUP * V - 1) / (GROUP * V));
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (i >= used) continue;
+            uint32_t start;
+            int skip;
+            at(i, lane, K, start, skip);
+            x[i].load(p + start);
+            if (skip > 0) {      // behind the row, or the pack that ends with it: a few threads of the last turn
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = j < skip ? -INFINITY : x[i].get(j);
+                x[i].set(v);
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (i >= used) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) f(x[i].get(j));
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void write(T* out, int lane, int64_t K, int64_t a, float more, F&& f) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (i >= used) continue;
+            uint32_t start;
+            int skip;
+            at(i, lane, K, start, skip);
+            if (skip < V) write_pack<T, V>(out, x[i], start, skip, a, more, f);
+        }
+    }
+};
+
+// A row that is not held: read for every use.
+template <typename E, int GROUP>
+struct Streamed {
+    using T = E;
+    static constexpr int kGroup = GROUP, kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr bool kHeld = false;
+    static constexpr int V = 16 / sizeof(T);
+    const T* row;
+    int64_t K;
+    int lane;
+
+    __device__ __forceinline__ void load(const T* p, int l, int64_t k) { row = p, lane = l, K = k; }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll 2
+        for (int64_t pack = lane; pack * V < K; pack += kGroup) {
+            int64_t start;
+            int skip;
+            place<V>(pack, K, start, skip);
+            Pack<T> x;
+            x.load(row + start);
+#pragma unroll
+            for (int j = 0; j < V; ++j) f(j >= skip ? x.get(j) : -INFINITY);
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void write(T* out, int l, int64_t k, int64_t a, float more, F&& f) const {
+#pragma unroll 2
+        for (int64_t pack = lane; pack * V < K; pack += kGroup) {
+            int64_t start;
+            int skip;
+            place<V>(pack, K, start, skip);
+            Pack<T> x;
+            x.load(row + start);
+            write_pack<T, V>(out, x, start, skip, a, more, f);
+        }
+    }
+};
+
+// The row that a thread begins with; uniform where a workgroup has one row.
+template <typename R>
+__device__ __forceinline__ int64_t first_row() {
+    constexpr int kRows = R::kThreads / R::kGroup;
+    return (int64_t)blockIdx.x * kRows + (kRows == 1 ? 0 : threadIdx.x / R::kGroup);
+}
+
+struct Stats {
+    float m, log_s, H;
+};
+
+// Maximum, then both sums. A row that is not held gathers them in one pass: a running maximum of a few logits at a
+// time rescales the sums when it grows.
+template <typename R>
+__device__ __forceinline__ Stats stats_of(const R& r, float* red) {
+    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    if constexpr (R::kHeld) {
+        r.each([&](float z) { m = fmaxf(m, z); });
+        m = group_max<R::kGroup>(m, red);
+        r.each([&](float z) {
+            const float d = z - m, e = exp_of(d);
+            s += e;
+            t += e * finite(d);
+        });
+    } else {
+        r.each([&](float z) {
+            if (z > m) {      // exp(-inf) = 0 rescales empty sums
+                const float d = m - z, e = exp_of(d);
+                t = e * (t + s * finite(d));
+                s *= e;
+                m = z;
+            }
+            const float d = z == -INFINITY ? z : z - m, e = exp_of(d);
+            s += e;
+            t += e * finite(d);
+        });
+        const float own = m;
+        m = group_max<R::kGroup>(m, red);
+        const float d = own == -INFINITY ? own : own - m, e = exp_of(d);
+        t = e * (t + s * finite(d));
+        s *= e;
+        if (m == -INFINITY) s = NAN;      // nothing can be taken
+    }
+    group_sums<R::kGroup>(s, t, red);
+    const float log_s = logf(s);
+    return {m, log_s, log_s - t / s};
+}
+
+template <typename R>
+__global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void log_probs_kernel(
+    int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ actions,
+    float* __restrict__ logp, float* __restrict__ ent, int32_t* __restrict__ bad) {
+    constexpr int kRows = R::kThreads / R::kGroup;
+    __shared__ float red[2 * R::kThreads / 64];
+    const int lane = R::kThreads == R::kGroup ? threadIdx.x : threadIdx.x % R::kGroup;
+    for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
+        R r;
+        r.load(logits + m * ld, lane, K);
+        const Stats st = stats_of(r, red);
+        if (lane == 0) {
+            const int64_t a = actions[m];
+            const bool in = a >= 0 && a < K;
+            logp[m] = in ? ((float)logits[m * ld + a] - st.m) - st.log_s : NAN;
+            ent[m] = st.H;
             if (!in && bad) atomicOr(bad, 1);
         }
     }
@@ -99,64 +303,158 @@ struct LossArgs {
     const float* ref_lp;
     const float* adv;
     const uint8_t* mask;
+    const float* denom;
     float lo, hi, kl_coef, ent_coef;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void loss_rows_kernel(int64_t M, int64_t K, const T* __restrict__ logits, int64_t ld,
-                                                             LossArgs p, float* __restrict__ row_stats,
-                                                             float* __restrict__ partials, int32_t* __restrict__ bad) {
-    __shared__ Stats red[kWaves];
-    float sums[kSums] = {};
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        if (p.mask && !p.mask[m]) {
-            if (threadIdx.x < 4) row_stats[4 * m + threadIdx.x] = 0.0f;
-            continue;
-        }
-        const T* z = logits + m * ld;
-        const Stats a = row_stats_of(z, K, red);
-        if (threadIdx.x != 0) continue;
-        const int64_t k = p.actions[m];
-        const bool in = k >= 0 && k < K;
-        if (!in && bad) atomicOr(bad, 1);
-        const float ls = logf(a.s);
-        const float l = in ? ((float)z[k] - a.m) - ls : NAN;
-        const float H = ls - a.t / a.s;
-        const float x = l - p.old_lp[m], A = p.adv[m];
-        const float r = expf(clamp_nan(x, -kBound, kBound));
-        const float u = r * A, v = clamp_nan(r, p.lo, p.hi) * A;
-        const float pg = u <= v ? -u : (u > v ? -v : u + v);
-        float g = (u <= v && x >= -kBound && x <= kBound) ? -u : (u > v ? 0.0f : u + v);
-        if (u <= v && !(x >= -kBound && x <= kBound)) g = 0.0f;
-        float kl = 0.0f;
-        if (p.ref_lp) {
-            const float y = p.ref_lp[m] - l, d = clamp_nan(y, -kBound, kBound), e = expf(d);
-            kl = e - d - 1.0f;
-            if (y >= -kBound && y <= kBound) g += p.kl_coef * (1.0f - e);
-        }
-        sums[0] += pg;
-        sums[1] += kl;
-        sums[2] += H;
-        sums[3] += (r < p.lo || r > p.hi) ? 1.0f : 0.0f;
-        sums[4] += pg + p.kl_coef * kl - p.ent_coef * H;
-        sums[5] += 1.0f;
-        row_stats[4 * m] = a.m + ls;
-        row_stats[4 * m + 1] = H;
-        row_stats[4 * m + 2] = g;
-        row_stats[4 * m + 3] = 1.0f;
-    }
-    if (threadIdx.x == 0)
-        for (int k = 0; k < kSums; ++k) partials[blockIdx.x * kSums + k] = sums[k];
+// active rows, by the whole workgroup, in every thread
+template <int THREADS>
+__device__ __forceinline__ float count_active(const uint8_t* mask, int64_t M, float* red) {
+    int n = 0;
+    for (int64_t m = threadIdx.x; m < M; m += THREADS) n += mask[m] ? 1 : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    int* r = reinterpret_cast<int*>(red);
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = 0;
+    for (int k = 0; k < THREADS / 64; ++k) n += r[k];
+    __syncthreads();
+    return (float)n;
 }
 
-__global__ __launch_bounds__(kThreads) void loss_finish_kernel(int blocks, int64_t M, int has_mask,
-                                                               const float* __restrict__ partials,
-                                                               const float* __restrict__ denom,
-                                                               float* __restrict__ loss, float* __restrict__ terms,
-                                                               float* __restrict__ used_denom) {
-    __shared__ double red[kWaves][kSums];
+__device__ __forceinline__ float at_least_one(float n) { return n > 1.0f ? n : 1.0f; }
+
+__global__ __launch_bounds__(1024) void loss_count_kernel(int64_t M, const uint8_t* __restrict__ mask,
+                                                          float* __restrict__ used_denom) {
+    int64_t n = 0;      // more rows than a 32-bit count
+    for (int64_t m = threadIdx.x; m < M; m += 1024) n += mask[m] ? 1 : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    __shared__ int64_t counts[1024 / 64];
+    if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int k = 1; k < 1024 / 64; ++k) n += counts[k];
+    *used_denom = at_least_one((float)n);
+}
+
+// What a row adds to the sums, and the gradient g of its terms in l.
+struct RowTerms {
+    float pg, kl, outside, g;
+};
+
+__device__ __forceinline__ RowTerms terms_of(const LossArgs& p, int64_t m, float l) {
+    RowTerms o;
+    const float x = l - p.old_lp[m], A = p.adv[m];
+    const float r = expf(clamp_nan(x, -kBound, kBound));
+    const float u = r * A, v = clamp_nan(r, p.lo, p.hi) * A;
+    const bool far = x < -kBound || x > kBound;
+    // u + v: NaN where either is. At a tie both sides of the minimum carry the gradient of u.
+    o.pg = u <= v ? -u : (u > v ? -v : u + v);
+    o.g = u <= v ? (far ? 0.0f : -u) : (u > v ? 0.0f : u + v);
+    o.outside = r < p.lo || r > p.hi ? 1.0f : 0.0f;
+    o.kl = 0.0f;
+    if (p.ref_lp) {
+        const float y = p.ref_lp[m] - l, d = clamp_nan(y, -kBound, kBound), e = expf(d);
+        o.kl = e - d - 1.0f;
+        if (!(y < -kBound || y > kBound)) o.g += p.kl_coef * (1.0f - e);
+    }
+    return o;
+}
+
+// p_k (c1 log p_k + c0): a row's gradient but for its action, with c1 = c entropy_coef, c0 = c (entropy_coef H - g)
+struct RowGrad {
+    float m, log_s, c1, c0;
+    __device__ __forceinline__ float operator()(float z) const {
+        const float lp = (z - m) - log_s;
+        return exp_of(lp) * (c1 * finite(lp) + c0);
+    }
+};
+
+template <typename R>
+__device__ __forceinline__ void zero_row(typename R::T* out, int lane, int64_t K) {
+    constexpr int V = 16 / sizeof(typename R::T);
+    Pack<typename R::T> none;
+    for (int j = 0; j < none.kWords; ++j) none.w[j] = 0u;
+    const int64_t packs = K / V;
+    for (int64_t k = lane; k < packs; k += R::kGroup) none.store(out + k * V);
+    for (int64_t k = packs * V + lane; k < K; k += R::kGroup) out[k] = (typename R::T)0.0f;
+}
+
+template <typename R>
+__global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void loss_rows_kernel(
+    int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, LossArgs p,
+    const float* __restrict__ counted, float* __restrict__ row_stats, float* __restrict__ partials,
+    typename R::T* __restrict__ dz, int32_t* __restrict__ bad) {
+    constexpr int kRows = R::kThreads / R::kGroup, W = R::kThreads / 64;
+    __shared__ float red[2 * W];
+    __shared__ float out[W][kSums];
+    const int lane = R::kThreads == R::kGroup ? threadIdx.x : threadIdx.x % R::kGroup;
+    float c = 0.0f;
+    if (dz) {
+        const float d = p.denom ? *p.denom
+                        : counted ? *counted
+                        : p.mask ? at_least_one(count_active<R::kThreads>(p.mask, M, red)) : (float)M;
+        c = 1.0f / d;
+    }
+    float sums[kSums] = {};
+    for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
+        R r;
+        const bool active = !p.mask || p.mask[m];
+        if (!active) {
+            if (lane == 0) {
+                row_stats[4 * m] = row_stats[4 * m + 2] = row_stats[4 * m + 3] = 0.0f;
+                row_stats[4 * m + 1] = kInactive;
+            }
+            if (dz) zero_row<R>(dz + m * K, lane, K);
+            continue;
+        }
+        r.load(logits + m * ld, lane, K);
+        const Stats st = stats_of(r, red);
+        const int64_t a = p.actions[m];
+        const bool in = a >= 0 && a < K;
+        const float l = in ? ((float)logits[m * ld + a] - st.m) - st.log_s : NAN;
+        const RowTerms t = terms_of(p, m, l);
+        if (lane == 0) {
+            if (!in && bad) atomicOr(bad, 1);
+            sums[0] += t.pg;
+            sums[1] += t.kl;
+            sums[2] += st.H;
+            sums[3] += t.outside;
+            sums[4] += t.pg + p.kl_coef * t.kl - p.ent_coef * st.H;
+            sums[5] += 1.0f;
+            row_stats[4 * m] = st.m;
+            row_stats[4 * m + 1] = st.log_s;
+            row_stats[4 * m + 2] = st.H;
+            row_stats[4 * m + 3] = t.g;
+        }
+        if (dz) {
+            const RowGrad f{st.m, st.log_s, c * p.ent_coef, c * (p.ent_coef * st.H - t.g)};
+            r.write(dz + m * K, lane, K, a, c * t.g, f);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sums[k] += __shfl_xor(sums[k], o);
+        if ((threadIdx.x & 63) == 0) out[threadIdx.x >> 6][k] = sums[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < kSums) {
+        float v = 0.0f;
+        for (int w = 0; w < W; ++w) v += out[w][threadIdx.x];
+        partials[blockIdx.x * kSums + threadIdx.x] = v;
+    }
+}
+
+__global__ __launch_bounds__(256) void loss_finish_kernel(int blocks, int64_t M, int has_mask,
+                                                          const float* __restrict__ partials,
+                                                          const float* __restrict__ denom, float* __restrict__ loss,
+                                                          float* __restrict__ terms, float* __restrict__ used_denom) {
+    __shared__ double red[4][kSums];
     double s[kSums] = {};
-    for (int b = threadIdx.x; b < blocks; b += kThreads)
+    for (int b = threadIdx.x; b < blocks; b += 256)
         for (int k = 0; k < kSums; ++k) s[k] += (double)partials[b * kSums + k];
     for (int k = 0; k < kSums; ++k) {
 #pragma unroll
@@ -166,38 +464,72 @@ __global__ __launch_bounds__(kThreads) void loss_finish_kernel(int blocks, int64
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int k = 0; k < kSums; ++k)
-        for (int w = 1; w < kWaves; ++w) s[k] += red[w][k];
-    const double n = has_mask ? s[5] : (double)M;
-    const double d = denom ? (double)*denom : (n > 1.0 ? n : 1.0);
-    *loss = (float)(s[4] / d);
-    for (int k = 0; k < 4; ++k) terms[k] = (float)(s[k] / d);
-    *used_denom = (float)d;
+        for (int w = 1; w < 4; ++w) s[k] += red[w][k];
+    const float n = has_mask ? (float)s[5] : (float)M;
+    const float d = denom ? *denom : at_least_one(n);
+    *loss = (float)(s[4] / (double)d);
+    for (int k = 0; k < 4; ++k) terms[k] = (float)(s[k] / (double)d);
+    *used_denom = d;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void loss_bwd_kernel(int64_t M, int64_t K, const T* __restrict__ logits, int64_t ld,
-                                                            const int64_t* __restrict__ actions, float ent_coef,
-                                                            const float* __restrict__ row_stats,
-                                                            const float* __restrict__ used_denom,
-                                                            const float* __restrict__ grad, T* __restrict__ dz) {
-    const float scale = *grad / *used_denom;
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-        const float L = row_stats[4 * m], H = row_stats[4 * m + 1], g = row_stats[4 * m + 2];
-        const bool active = row_stats[4 * m + 3] != 0.0f;
-        const int64_t a = actions[m];
-        for (int64_t k = threadIdx.x; k < K; k += kThreads) {
-            float d = 0.0f;
-            if (active) {
-                const float lp = (float)logits[m * ld + k] - L, q = exp_of(lp);
-                d = g * ((k == a ? 1.0f : 0.0f) - q) + (q == 0.0f ? 0.0f : ent_coef * q * (lp + H));
-                d *= scale;
-            }
-            dz[m * K + k] = (T)d;
+template <typename R>
+__global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
+    int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ actions,
+    float ent_coef, const float* __restrict__ row_stats, const float* __restrict__ used_denom,
+    const float* __restrict__ grad, int have, typename R::T* __restrict__ dz) {
+    constexpr int kRows = R::kThreads / R::kGroup;
+    const float g = *grad;
+    if (have && g == 1.0f) return;
+    const float c = g / *used_denom;
+    const int lane = R::kThreads == R::kGroup ? threadIdx.x : threadIdx.x % R::kGroup;
+    for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
+        const float mx = row_stats[4 * m], log_s = row_stats[4 * m + 1], H = row_stats[4 * m + 2];
+        const float gl = row_stats[4 * m + 3];
+        if (log_s == kInactive) {
+            zero_row<R>(dz + m * K, lane, K);
+            continue;
         }
+        R r;
+        r.load(logits + m * ld, lane, K);
+        const RowGrad f{mx, log_s, c * ent_coef, c * (ent_coef * H - gl)};
+        r.write(dz + m * K, lane, K, actions[m], c * gl, f);
     }
 }
 
-unsigned blocks_of(int64_t M) { return (unsigned)(M < kMaxBlocks ? M : kMaxBlocks); }
+// The fewest threads that hold a row of K logits, calls fn with its layout.
+template <typename T, typename F>
+void with_layout(int64_t K, F&& fn) {
+    if (K <= 8) fn(Narrow<T, 1, 8>{});
+    else if (K <= 64) fn(Narrow<T, 8, 8>{});
+    else if (K <= 512) fn(Narrow<T, 64, 8>{});
+    else if (K <= 2048) fn(Wide<T, 64, 32>{});
+    else if (K <= 8192) fn(Wide<T, 256, 32>{});
+    else if (K <= 32768) fn(Wide<T, 512, 64>{});
+    else if constexpr (sizeof(T) == 2) {
+        if (K <= 65536) fn(Wide<T, 512, 128>{});
+        else if (K <= 131072) fn(Wide<T, 1024, 128>{});
+        else fn(Streamed<T, 1024>{});
+    } else {
+        if (K <= 65536) fn(Wide<T, 1024, 64>{});
+        else fn(Streamed<T, 1024>{});
+    }
+}
+
+// For one use of a row.
+template <typename T, typename F>
+void with_pass(int64_t K, F&& fn) {
+    if (K <= 8) fn(Narrow<T, 1, 8>{});
+    else if (K <= 64) fn(Narrow<T, 8, 8>{});
+    else if (K <= 512) fn(Narrow<T, 64, 8>{});
+    else if (K <= 2048) fn(Streamed<T, 64>{});
+    else fn(Streamed<T, 256>{});
+}
+
+template <typename R>
+unsigned grid_of(int64_t M, int64_t most) {
+    const int64_t rows = R::kThreads / R::kGroup, b = (M + rows - 1) / rows;
+    return (unsigned)(b < most ? b : most);
+}
 
 }  // namespace
 
@@ -210,8 +542,11 @@ int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits,
     if (!logits || !actions || !log_probs || !entropy || row_stride < 0) return SWARM_ERR_ARG;
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        log_probs_kernel<E><<<(unsigned)(M < 65536 ? M : 65536), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            M, K, static_cast<const E*>(logits), row_stride, actions, log_probs, entropy, bad_actions);
+        with_layout<E>(K, [&](auto layout) {
+            using R = decltype(layout);
+            log_probs_kernel<R><<<grid_of<R>(M, 1 << 20), R::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                M, K, static_cast<const E*>(logits), row_stride, actions, log_probs, entropy, bad_actions);
+        });
     });
     return swarm::record_hip_status();
 }
@@ -220,40 +555,50 @@ int32_t swarm_policy_loss_forward(int32_t dtype, int64_t M, int64_t K, const voi
                                   const int64_t* actions, const float* old_log_probs, const float* ref_log_probs,
                                   const float* advantages, const uint8_t* mask_u8, const float* denom, float clip_lo,
                                   float clip_hi, float kl_coef, float entropy_coef, float* loss, float* terms,
-                                  float* used_denom, float* row_stats, float* partials, int32_t* bad_actions,
-                                  void* stream) {
+                                  float* used_denom, float* row_stats, void* d_logits, float* partials,
+                                  int32_t* bad_actions, void* stream) {
     if (!known_type(dtype) || M < 0 || K < 1 || !sane(M, K) || !loss || !terms || !used_denom || !partials ||
         !(clip_lo <= clip_hi))
         return SWARM_ERR_ARG;
     if (M > 0 && (!logits || !actions || !old_log_probs || !advantages || !row_stats || row_stride < 0))
         return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const unsigned blocks = blocks_of(M);
+    unsigned blocks = 0;
     if (M > 0) {
-        const LossArgs p{actions, old_log_probs, ref_log_probs, advantages, mask_u8, clip_lo, clip_hi, kl_coef,
+        const LossArgs p{actions, old_log_probs, ref_log_probs, advantages, mask_u8, denom, clip_lo, clip_hi, kl_coef,
                          entropy_coef};
+        const bool count = d_logits && mask_u8 && !denom && M > kCountHere;
+        if (count) loss_count_kernel<<<1, 1024, 0, st>>>(M, mask_u8, used_denom);
         with_type(dtype, [&](auto e) {
             using E = decltype(e);
-            loss_rows_kernel<E><<<blocks, kThreads, 0, st>>>(M, K, static_cast<const E*>(logits), row_stride, p,
-                                                            row_stats, partials, bad_actions);
+            with_layout<E>(K, [&](auto layout) {
+                using R = decltype(layout);
+                blocks = grid_of<R>(M, kMaxBlocks);
+                loss_rows_kernel<R><<<blocks, R::kThreads, 0, st>>>(M, K, static_cast<const E*>(logits), row_stride, p,
+                                                                  count ? used_denom : nullptr, row_stats, partials,
+                                                                  static_cast<E*>(d_logits), bad_actions);
+            });
         });
     }
-    loss_finish_kernel<<<1, kThreads, 0, st>>>((int)blocks, M, mask_u8 != nullptr, partials, denom, loss, terms,
-                                              used_denom);
+    loss_finish_kernel<<<1, 256, 0, st>>>((int)blocks, M, mask_u8 != nullptr, partials, denom, loss, terms, used_denom);
     return swarm::record_hip_status();
 }
 
 int32_t swarm_policy_loss_backward(int32_t dtype, int64_t M, int64_t K, const void* logits, int64_t row_stride,
                                    const int64_t* actions, float entropy_coef, const float* row_stats,
-                                   const float* used_denom, const float* grad, void* d_logits, void* stream) {
+                                   const float* used_denom, const float* grad, int32_t have_unit, void* d_logits,
+                                   void* stream) {
     if (!known_type(dtype) || M < 0 || K < 1 || !sane(M, K)) return SWARM_ERR_ARG;
     if (M == 0) return SWARM_OK;
     if (!logits || !actions || !row_stats || !used_denom || !grad || !d_logits || row_stride < 0) return SWARM_ERR_ARG;
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        loss_bwd_kernel<E><<<(unsigned)(M < 65536 ? M : 65536), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            M, K, static_cast<const E*>(logits), row_stride, actions, entropy_coef, row_stats, used_denom, grad,
-            static_cast<E*>(d_logits));
+        with_pass<E>(K, [&](auto layout) {
+            using R = decltype(layout);
+            loss_bwd_kernel<R><<<grid_of<R>(M, kMaxBlocks), R::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                M, K, static_cast<const E*>(logits), row_stride, actions, entropy_coef, row_stats, used_denom, grad,
+                have_unit, static_cast<E*>(d_logits));
+        });
     });
     return swarm::record_hip_status();
 }

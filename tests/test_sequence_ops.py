@@ -213,13 +213,13 @@ def test_c_abi_refusals():
         assert lp(**kw) == -1, kw
     lf = lambda dt=0, M=1, K=1, z=p, a=p, old=p, adv=p, lo=0.8, hi=1.2, loss=p, terms=p, used=p, st=p, part=p: (  # noqa: E731
         lib.swarm_policy_loss_forward(dt, M, K, z, 1, a, old, None, adv, None, None, lo, hi, 0.0, 0.0, loss, terms,
-                                      used, st, part, None, None))
+                                      used, st, None, part, None, None))
     for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(old=None), dict(adv=None),
                dict(lo=1.3), dict(lo=float("nan")), dict(loss=None), dict(terms=None), dict(used=None), dict(st=None),
                dict(part=None)):
         assert lf(**kw) == -1, kw
     lb = lambda dt=0, M=1, K=1, z=p, a=p, st=p, used=p, g=p, d=p: lib.swarm_policy_loss_backward(  # noqa: E731
-        dt, M, K, z, 1, a, 0.0, st, used, g, d, None)
+        dt, M, K, z, 1, a, 0.0, st, used, g, 0, d, None)
     assert lb(M=0) == 0
     for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(st=None), dict(used=None),
                dict(g=None), dict(d=None)):
