@@ -1,11 +1,13 @@
 // swarm_policyloss.hip — log-probabilities and the clipped policy loss with a KL term, from logits
 // (include/swarmseq.h: swarm_log_probs, swarm_policy_loss_*).
 //
-// Per row of K logits z with the taken action a, m = max z, d_k = z_k - m, s = sum exp d_k, t = sum exp(d_k) d_k:
-//   log p_k = d_k - log s,  l = log p_a,  H = log s - t / s
+// Per row of K logits z with the taken action a, m = max z, x_k = (z_k - m) log2 e, e_k = 2^x_k, s = sum e_k,
+// t = sum e_k x_k:
+//   log p_k = x_k ln 2 - log s,  p_k = e_k / s,  l = log p_a,  H = log s - (t / s) ln 2
 //   dz_k = c [ g (1[k = a] - p_k) + entropy_coef p_k (log p_k + H) ],   c = incoming gradient / denominator,
 //   g = d pg / d l + kl_coef (1 - exp(ref - l)).
-// A logit of -inf adds nothing to either sum and has no gradient: its exp is 0, and so are the products it enters.
+// x is held above -200, where e is 0 in float32: a logit of -inf adds nothing to either sum and has no gradient. A
+// NaN or an infinite maximum would be lost there, so such a row's s is set to NaN.
 //
 // Memory bound. A row is read once and held in registers by as many threads as it needs; maximum, then both sums,
 // are reduced over them. Since the denominator does not depend on the logits, the gradient for an incoming gradient
@@ -23,13 +25,14 @@ namespace {
 constexpr int kMaxBlocks = 2048;      // SWARM_POLICY_LOSS_PARTIALS = kSums for each
 constexpr int kSums = 6;              // pg, kl, H, outside, pg + kl_coef kl - entropy_coef H, active rows
 constexpr float kBound = 20.0f;       // bound of the log-ratios
-constexpr float kInactive = -1.0f;    // log s of a row that takes no part (log s >= 0 elsewhere: exp d = 1 at the maximum)
-constexpr int64_t kCountHere = 8192;  // masks up to this many rows are counted by every workgroup itself
+constexpr float kInactive = -1.0f;    // s of a row that takes no part (s >= 1 elsewhere: e = 1 at the maximum)
+constexpr unsigned kCountHere = 256;  // up to this many workgroups, each counts the active rows itself
 
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+constexpr float kLn2 = 0.69314718055994530942f;
 
-// An exponent as a factor: finite, so that 0 = exp(-inf) times it is 0. (A NaN is dropped here; its exp is the NaN.)
-__device__ __forceinline__ float finite(float d) { return fmaxf(d, -1e30f); }
+__device__ __forceinline__ float exponent(float z, float m) { return fmaxf((z - m) * kLog2e, -200.0f); }
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // clamp that keeps a NaN
 __device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return x < lo ? lo : (x > hi ? hi : x); }
@@ -37,26 +40,22 @@ __device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return
 // Reductions over a row's GROUP threads, in every one.
 template <int GROUP>
 __device__ __forceinline__ float group_max(float v, float* red) {
-#pragma unroll
-    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    v = lanes_reduce<(GROUP < 64 ? GROUP : 64)>(v, Maximum{});
     if constexpr (GROUP > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = red[0];
 #pragma unroll
-        for (int k = 1; k < GROUP / 64; ++k) v = fmaxf(v, red[k]);
+        for (int k = 1; k < GROUP / 64; ++k) v = Maximum{}(v, red[k]);
     }
     return v;
 }
 
 template <int GROUP>
 __device__ __forceinline__ void group_sums(float& s, float& t, float* red) {
-#pragma unroll
-    for (int o = (GROUP < 64 ? GROUP : 64) / 2; o > 0; o >>= 1) {
-        s += __shfl_xor(s, o);
-        t += __shfl_xor(t, o);
-    }
+    s = lanes_reduce<(GROUP < 64 ? GROUP : 64)>(s, Add{});
+    t = lanes_reduce<(GROUP < 64 ? GROUP : 64)>(t, Add{});
     if constexpr (GROUP > 64) {
         constexpr int W = GROUP / 64;
         __syncthreads();
@@ -75,6 +74,8 @@ struct Narrow {
     static constexpr int kGroup = LPR, kThreads = 256;
     static constexpr bool kHeld = true;
     float z[N];
+    static size_t lds_bytes(int64_t) { return 0; }
+
 
     __device__ __forceinline__ void load(const T* p, int lane, int64_t K) {
 #pragma unroll
@@ -85,20 +86,22 @@ struct Narrow {
 #pragma unroll
         for (int i = 0; i < N; ++i) z[i] = lane + i * LPR < (int)K ? z[i] : -INFINITY;
     }
+    // f of all values, a few at a time
     template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) f(z[i]);
+    __device__ __forceinline__ void each(int, F&& f) const {
+        f(z);
     }
-    // out[k] = f(z_k), and more at the action
+    // out[k] = f(z_k)
     template <typename F>
-    __device__ __forceinline__ void write(T* out, int lane, int64_t K, int64_t a, float more, F&& f) const {
+    __device__ __forceinline__ void write(T* out, int lane, int64_t K, F&& f) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int k = lane + i * LPR;
-            if (k < (int)K) out[k] = (T)(f(z[i]) + (k == a ? more : 0.0f));
+            if (k < (int)K) out[k] = (T)f(z[i]);
         }
     }
+    // the thread that stores an element
+    static __device__ __forceinline__ int owner(int64_t a) { return (int)a % LPR; }
 };
 
 // Pack i of a thread of a long row: its first column, and how many of its elements belong to the pack before (the
@@ -110,99 +113,125 @@ __device__ __forceinline__ void place(int64_t pack, int64_t K, int64_t& start, i
     skip = want - start < V ? (int)(want - start) : V;
 }
 
-// Stores f of a pack's own elements, and more at the action.
+// Stores f of a pack's own elements.
 template <typename T, int V, typename F>
-__device__ __forceinline__ void write_pack(T* out, const Pack<T>& x, int64_t start, int skip, int64_t a, float more,
-                                           F&& f) {
+__device__ __forceinline__ void write_pack(T* out, const Pack<T>& x, int skip, F&& f) {
     float v[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = f(x.get(j));
-    const uint64_t at = (uint64_t)(a - start);
-    if (at < (uint64_t)V) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += at == (uint64_t)j ? more : 0.0f;
-    }
     Pack<T> w;
     w.set(v);
     if (skip == 0) {
-        w.store(out + start);
+        w.store(out);
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (j >= skip) out[start + j] = (T)w.get(j);
+            if (j >= skip) out[j] = (T)w.get(j);
     }
 }
 
-// A longer row: EPT logits of each of GROUP threads, in packs of 16 bytes at any alignment.
-template <typename E, int GROUP, int EPT>
+// A longer row: EPT logits of each of GROUP threads in registers, in packs of 16 bytes at any alignment, and up to
+// EXTRA more packs of each in LDS, where only their own thread reads them.
+template <typename E, int GROUP, int EPT, int EXTRA = 0>
 struct Wide {
     using T = E;
-    static constexpr int kGroup = GROUP, kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr int kGroup = GROUP, kThreads = GROUP <= 64 ? 256 : GROUP;
     static constexpr bool kHeld = true;
     static constexpr int V = 16 / sizeof(T), NP = EPT / V;
+    static constexpr int64_t kMost = (int64_t)GROUP * V * (NP + EXTRA);
     Pack<T> x[NP];
     int used;      // packs of a thread that any thread needs
 
-    // as place(), in 32 bits: one register an address, next to the row's uniform base
-    static __device__ __forceinline__ void at(int i, int lane, int64_t K, uint32_t& start, int& skip) {
+    static size_t lds_bytes(int64_t K) {
+        const int64_t packs = (K + GROUP * V - 1) / (GROUP * V);
+        return EXTRA > 0 && packs > NP ? (size_t)(packs - NP) * GROUP * 16 : 0;
+    }
+    static __device__ __forceinline__ Pack<T>* extra(int i, int lane) {
+        extern __shared__ __align__(16) uint32_t row_lds[];
+        return reinterpret_cast<Pack<T>*>(row_lds) + (i - NP) * GROUP + lane;
+    }
+
+    // Pack i's first column, in 32 bits: one register an address, next to the row's uniform base.
+    static __device__ __forceinline__ uint32_t column(int i, int lane, int64_t K) {
         const uint32_t want = (uint32_t)(i * GROUP + lane) * V, last = (uint32_t)K - V;
-        start = want < last ? want : last;
-        skip = want - start < (uint32_t)V ? (int)(want - start) : V;
+        return want < last ? want : last;
+    }
+    // What a thread leaves out of its last pack: only packs of the last turn can reach behind the row.
+    __device__ __forceinline__ int skipped(int lane, int64_t K) const {
+        const uint32_t want = (uint32_t)((used - 1) * GROUP + lane) * V, start = column(used - 1, lane, K);
+        return want - start < (uint32_t)V ? (int)(want - start) : V;
+    }
+
+    __device__ __forceinline__ Pack<T> fetch(const T* p, int i, int lane, int64_t K, int skip) const {
+        Pack<T> x;
+        x.load(p + column(i, lane, K));
+        if (i == used - 1) {
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = j < skip ? -INFINITY : x.get(j);
+            x.set(v);
+        }
+        return x;
     }
 
     __device__ __forceinline__ void load(const T* p, int lane, int64_t K) {
         used = (int)((K + GROUP * V - 1) / (GROUP * V));
+        const int skip = skipped(lane, K);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            if (i >= used) continue;
-            uint32_t start;
-            int skip;
-            at(i, lane, K, start, skip);
-            x[i].load(p + start);
-            if (skip > 0) {      // behind the row, or the pack that ends with it: a few threads of the last turn
-                float v[V];
+        for (int i = 0; i < NP; ++i)
+            if (i < used) x[i] = fetch(p, i, lane, K, skip);
+        if constexpr (EXTRA > 0) {
+            Pack<T> y[EXTRA];
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = j < skip ? -INFINITY : x[i].get(j);
-                x[i].set(v);
-            }
+            for (int i = NP; i < NP + EXTRA; ++i)
+                if (i < used) y[i - NP] = fetch(p, i, lane, K, skip);
+#pragma unroll
+            for (int i = NP; i < NP + EXTRA; ++i)
+                if (i < used) *extra(i, lane) = y[i - NP];
         }
     }
     template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
+    __device__ __forceinline__ void each(int lane, F&& f) const {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
+        for (int i = 0; i < NP + EXTRA; ++i) {
             if (i >= used) continue;
+            float v[V];
+            const Pack<T> y = i < NP ? x[i < NP ? i : 0] : *extra(i, lane);
 #pragma unroll
-            for (int j = 0; j < V; ++j) f(x[i].get(j));
+            for (int j = 0; j < V; ++j) v[j] = y.get(j);
+            f(v);
         }
     }
     template <typename F>
-    __device__ __forceinline__ void write(T* out, int lane, int64_t K, int64_t a, float more, F&& f) const {
+    __device__ __forceinline__ void write(T* out, int lane, int64_t K, F&& f) const {
+        const int skip = skipped(lane, K);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
+        for (int i = 0; i < NP + EXTRA; ++i) {
             if (i >= used) continue;
-            uint32_t start;
-            int skip;
-            at(i, lane, K, start, skip);
-            if (skip < V) write_pack<T, V>(out, x[i], start, skip, a, more, f);
+            const Pack<T> y = i < NP ? x[i < NP ? i : 0] : *extra(i, lane);
+            T* to = out + column(i, lane, K);
+            if (i < used - 1) write_pack<T, V>(to, y, 0, f);
+            else if (skip < V) write_pack<T, V>(to, y, skip, f);
         }
     }
+    static __device__ __forceinline__ int owner(int64_t a) { return (int)(a / V % GROUP); }
 };
 
 // A row that is not held: read for every use.
 template <typename E, int GROUP>
 struct Streamed {
     using T = E;
-    static constexpr int kGroup = GROUP, kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr int kGroup = GROUP, kThreads = GROUP <= 64 ? 256 : GROUP;
     static constexpr bool kHeld = false;
     static constexpr int V = 16 / sizeof(T);
     const T* row;
     int64_t K;
     int lane;
+    static size_t lds_bytes(int64_t) { return 0; }
 
     __device__ __forceinline__ void load(const T* p, int l, int64_t k) { row = p, lane = l, K = k; }
     template <typename F>
-    __device__ __forceinline__ void each(F&& f) const {
+    __device__ __forceinline__ void each(int, F&& f) const {
 #pragma unroll 2
         for (int64_t pack = lane; pack * V < K; pack += kGroup) {
             int64_t start;
@@ -210,12 +239,14 @@ struct Streamed {
             place<V>(pack, K, start, skip);
             Pack<T> x;
             x.load(row + start);
+            float v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) f(j >= skip ? x.get(j) : -INFINITY);
+            for (int j = 0; j < V; ++j) v[j] = j >= skip ? x.get(j) : -INFINITY;
+            f(v);
         }
     }
     template <typename F>
-    __device__ __forceinline__ void write(T* out, int l, int64_t k, int64_t a, float more, F&& f) const {
+    __device__ __forceinline__ void write(T* out, int, int64_t, F&& f) const {
 #pragma unroll 2
         for (int64_t pack = lane; pack * V < K; pack += kGroup) {
             int64_t start;
@@ -223,9 +254,10 @@ struct Streamed {
             place<V>(pack, K, start, skip);
             Pack<T> x;
             x.load(row + start);
-            write_pack<T, V>(out, x, start, skip, a, more, f);
+            write_pack<T, V>(out + start, x, skip, f);
         }
     }
+    static __device__ __forceinline__ int owner(int64_t a) { return (int)(a / V % GROUP); }
 };
 
 // The row that a thread begins with; uniform where a workgroup has one row.
@@ -236,44 +268,68 @@ __device__ __forceinline__ int64_t first_row() {
 }
 
 struct Stats {
-    float m, log_s, H;
+    float m, s, log_s, H;
 };
 
-// Maximum, then both sums. A row that is not held gathers them in one pass: a running maximum of a few logits at a
-// time rescales the sums when it grows.
+// Maximum, then both sums. A row that is not held gathers them in one pass: a running maximum rescales the sums when
+// it grows.
 template <typename R>
-__device__ __forceinline__ Stats stats_of(const R& r, float* red) {
+__device__ __forceinline__ Stats stats_of(const R& r, int lane, float* red) {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
+    auto largest = [](const auto& v, float m) {
+#pragma unroll
+        for (unsigned j = 0; j < sizeof(v) / sizeof(float); ++j) m = Maximum{}(m, v[j]);
+        return m;
+    };
+    auto add = [&](const auto& v) {
+#pragma unroll
+        for (unsigned j = 0; j < sizeof(v) / sizeof(float); ++j) {
+            const float x = exponent(v[j], m), e = exp2_of(x);
+            s += e;
+            t += e * x;
+        }
+    };
     if constexpr (R::kHeld) {
-        r.each([&](float z) { m = fmaxf(m, z); });
+        r.each(lane, [&](const auto& v) { m = largest(v, m); });
         m = group_max<R::kGroup>(m, red);
-        r.each([&](float z) {
-            const float d = z - m, e = exp_of(d);
-            s += e;
-            t += e * finite(d);
-        });
+        r.each(lane, add);
     } else {
-        r.each([&](float z) {
-            if (z > m) {      // exp(-inf) = 0 rescales empty sums
-                const float d = m - z, e = exp_of(d);
-                t = e * (t + s * finite(d));
-                s *= e;
-                m = z;
-            }
-            const float d = z == -INFINITY ? z : z - m, e = exp_of(d);
-            s += e;
-            t += e * finite(d);
+        auto rescale = [&](float to) {
+            const float x = exponent(m, to), e = exp2_of(x);
+            t = e * (t + x * s);
+            s *= e;
+            m = to;
+        };
+        r.each(lane, [&](const auto& v) {
+            const float to = largest(v, m);
+            if (!(to <= m)) rescale(to);
+            add(v);
         });
-        const float own = m;
-        m = group_max<R::kGroup>(m, red);
-        const float d = own == -INFINITY ? own : own - m, e = exp_of(d);
-        t = e * (t + s * finite(d));
-        s *= e;
-        if (m == -INFINITY) s = NAN;      // nothing can be taken
+        rescale(group_max<R::kGroup>(m, red));
     }
     group_sums<R::kGroup>(s, t, red);
+    if (!(fabsf(m) < INFINITY)) s = NAN;
     const float log_s = logf(s);
-    return {m, log_s, log_s - t / s};
+    return {m, s, log_s, log_s - t * __builtin_amdgcn_rcpf(s) * kLn2};
+}
+
+// log p of a logit
+__device__ __forceinline__ float log_prob(const Stats& st, float z) { return (z - st.m) - st.log_s; }
+
+// A row's action and its logit.
+struct Taken {
+    int64_t a;
+    float z;
+    bool in;
+};
+
+template <typename T>
+__device__ __forceinline__ Taken taken_of(const int64_t* actions, int64_t m, const T* row, int64_t K) {
+    Taken t;
+    t.a = actions[m];
+    t.in = t.a >= 0 && t.a < K;
+    t.z = (float)row[t.in ? t.a : 0];
+    return t;
 }
 
 template <typename R>
@@ -286,13 +342,12 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void log_p
     for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
         R r;
         r.load(logits + m * ld, lane, K);
-        const Stats st = stats_of(r, red);
+        const Taken a = taken_of(actions, m, logits + m * ld, K);
+        const Stats st = stats_of(r, lane, red);
         if (lane == 0) {
-            const int64_t a = actions[m];
-            const bool in = a >= 0 && a < K;
-            logp[m] = in ? ((float)logits[m * ld + a] - st.m) - st.log_s : NAN;
+            logp[m] = a.in ? log_prob(st, a.z) : NAN;
             ent[m] = st.H;
-            if (!in && bad) atomicOr(bad, 1);
+            if (!a.in && bad) atomicOr(bad, 1);
         }
     }
 }
@@ -327,8 +382,16 @@ __device__ __forceinline__ float at_least_one(float n) { return n > 1.0f ? n : 1
 
 __global__ __launch_bounds__(1024) void loss_count_kernel(int64_t M, const uint8_t* __restrict__ mask,
                                                           float* __restrict__ used_denom) {
-    int64_t n = 0;      // more rows than a 32-bit count
-    for (int64_t m = threadIdx.x; m < M; m += 1024) n += mask[m] ? 1 : 0;
+    int64_t n = 0;
+    const int64_t packs = M / 16;
+    for (int64_t k = threadIdx.x; k < packs; k += 1024) {
+        uint32_t w[4];
+        __builtin_memcpy(w, mask + 16 * k, 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)      // the top bit of every byte that is not 0
+            n += __builtin_popcount((((w[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[j]) & 0x80808080u);
+    }
+    for (int64_t m = packs * 16 + threadIdx.x; m < M; m += 1024) n += mask[m] ? 1 : 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
     __shared__ int64_t counts[1024 / 64];
@@ -339,14 +402,25 @@ __global__ __launch_bounds__(1024) void loss_count_kernel(int64_t M, const uint8
     *used_denom = at_least_one((float)n);
 }
 
+// A row's operands, fetched one row ahead.
+struct RowIn {
+    bool active;
+    float old_lp, ref_lp, adv;
+};
+
+__device__ __forceinline__ RowIn row_in(const LossArgs& p, int64_t m, int64_t M) {
+    const int64_t k = m < M ? m : M - 1;
+    return {!p.mask || p.mask[k], p.old_lp[k], p.ref_lp ? p.ref_lp[k] : 0.0f, p.adv[k]};
+}
+
 // What a row adds to the sums, and the gradient g of its terms in l.
 struct RowTerms {
     float pg, kl, outside, g;
 };
 
-__device__ __forceinline__ RowTerms terms_of(const LossArgs& p, int64_t m, float l) {
+__device__ __forceinline__ RowTerms terms_of(const LossArgs& p, const RowIn& in, float l) {
     RowTerms o;
-    const float x = l - p.old_lp[m], A = p.adv[m];
+    const float x = l - in.old_lp, A = in.adv;
     const float r = expf(clamp_nan(x, -kBound, kBound));
     const float u = r * A, v = clamp_nan(r, p.lo, p.hi) * A;
     const bool far = x < -kBound || x > kBound;
@@ -356,21 +430,34 @@ __device__ __forceinline__ RowTerms terms_of(const LossArgs& p, int64_t m, float
     o.outside = r < p.lo || r > p.hi ? 1.0f : 0.0f;
     o.kl = 0.0f;
     if (p.ref_lp) {
-        const float y = p.ref_lp[m] - l, d = clamp_nan(y, -kBound, kBound), e = expf(d);
+        const float y = in.ref_lp - l, d = clamp_nan(y, -kBound, kBound), e = expf(d);
         o.kl = e - d - 1.0f;
         if (!(y < -kBound || y > kBound)) o.g += p.kl_coef * (1.0f - e);
     }
     return o;
 }
 
-// p_k (c1 log p_k + c0): a row's gradient but for its action, with c1 = c entropy_coef, c0 = c (entropy_coef H - g)
+// p_k c (entropy_coef (log p_k + H) - g) = e_k (c1 x_k + c0): a row's gradient but for its action
 struct RowGrad {
-    float m, log_s, c1, c0;
+    float m, c1, c0;
+    __device__ __forceinline__ RowGrad(float m, float s, float log_s, float H, float g, float c, float ent_coef) : m(m) {
+        const float share = __builtin_amdgcn_rcpf(s), ce = c * ent_coef;
+        c1 = ce * kLn2 * share;
+        c0 = (ce * (H - log_s) - c * g) * share;
+    }
     __device__ __forceinline__ float operator()(float z) const {
-        const float lp = (z - m) - log_s;
-        return exp_of(lp) * (c1 * finite(lp) + c0);
+        const float x = exponent(z, m);
+        return exp2_of(x) * (c1 * x + c0);
     }
 };
+
+// A row's gradient. The action's element is stored once more, with its own term, by the thread that stored it.
+template <typename R>
+__device__ __forceinline__ void write_grad(const R& r, typename R::T* out, int lane, int64_t K, const Taken& a,
+                                           float more, const RowGrad& f) {
+    r.write(out, lane, K, f);
+    if (a.in && lane == R::owner(a.a)) out[a.a] = (typename R::T)(f(a.z) + more);
+}
 
 template <typename R>
 __device__ __forceinline__ void zero_row(typename R::T* out, int lane, int64_t K) {
@@ -383,7 +470,7 @@ __device__ __forceinline__ void zero_row(typename R::T* out, int lane, int64_t K
 }
 
 template <typename R>
-__global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void loss_rows_kernel(
+__global__ __launch_bounds__(R::kThreads, R::kThreads >= 256 ? 4 : 0) void loss_rows_kernel(
     int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, LossArgs p,
     const float* __restrict__ counted, float* __restrict__ row_stats, float* __restrict__ partials,
     typename R::T* __restrict__ dz, int32_t* __restrict__ bad) {
@@ -399,10 +486,11 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void loss_
         c = 1.0f / d;
     }
     float sums[kSums] = {};
+    RowIn next = row_in(p, first_row<R>(), M);
     for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
-        R r;
-        const bool active = !p.mask || p.mask[m];
-        if (!active) {
+        const RowIn in = next;
+        next = row_in(p, m + (int64_t)gridDim.x * kRows, M);
+        if (!in.active) {
             if (lane == 0) {
                 row_stats[4 * m] = row_stats[4 * m + 2] = row_stats[4 * m + 3] = 0.0f;
                 row_stats[4 * m + 1] = kInactive;
@@ -410,14 +498,13 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void loss_
             if (dz) zero_row<R>(dz + m * K, lane, K);
             continue;
         }
+        R r;
         r.load(logits + m * ld, lane, K);
-        const Stats st = stats_of(r, red);
-        const int64_t a = p.actions[m];
-        const bool in = a >= 0 && a < K;
-        const float l = in ? ((float)logits[m * ld + a] - st.m) - st.log_s : NAN;
-        const RowTerms t = terms_of(p, m, l);
+        const Taken a = taken_of(p.actions, m, logits + m * ld, K);
+        const Stats st = stats_of(r, lane, red);
+        const RowTerms t = terms_of(p, in, a.in ? log_prob(st, a.z) : NAN);
         if (lane == 0) {
-            if (!in && bad) atomicOr(bad, 1);
+            if (!a.in && bad) atomicOr(bad, 1);
             sums[0] += t.pg;
             sums[1] += t.kl;
             sums[2] += st.H;
@@ -425,14 +512,11 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void loss_
             sums[4] += t.pg + p.kl_coef * t.kl - p.ent_coef * st.H;
             sums[5] += 1.0f;
             row_stats[4 * m] = st.m;
-            row_stats[4 * m + 1] = st.log_s;
+            row_stats[4 * m + 1] = st.s;
             row_stats[4 * m + 2] = st.H;
             row_stats[4 * m + 3] = t.g;
         }
-        if (dz) {
-            const RowGrad f{st.m, st.log_s, c * p.ent_coef, c * (p.ent_coef * st.H - t.g)};
-            r.write(dz + m * K, lane, K, a, c * t.g, f);
-        }
+        if (dz) write_grad(r, dz + m * K, lane, K, a, c * t.g, RowGrad(st.m, st.s, st.log_s, st.H, t.g, c, p.ent_coef));
     }
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
@@ -483,36 +567,37 @@ __global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
     const float c = g / *used_denom;
     const int lane = R::kThreads == R::kGroup ? threadIdx.x : threadIdx.x % R::kGroup;
     for (int64_t m = first_row<R>(); m < M; m += (int64_t)gridDim.x * kRows) {
-        const float mx = row_stats[4 * m], log_s = row_stats[4 * m + 1], H = row_stats[4 * m + 2];
+        const float mx = row_stats[4 * m], s = row_stats[4 * m + 1], H = row_stats[4 * m + 2];
         const float gl = row_stats[4 * m + 3];
-        if (log_s == kInactive) {
+        if (s == kInactive) {
             zero_row<R>(dz + m * K, lane, K);
             continue;
         }
         R r;
         r.load(logits + m * ld, lane, K);
-        const RowGrad f{mx, log_s, c * ent_coef, c * (ent_coef * H - gl)};
-        r.write(dz + m * K, lane, K, actions[m], c * gl, f);
+        write_grad(r, dz + m * K, lane, K, taken_of(actions, m, logits + m * ld, K), c * gl,
+                   RowGrad(mx, s, logf(s), H, gl, c, ent_coef));
     }
 }
 
-// The fewest threads that hold a row of K logits, calls fn with its layout.
+// The fewest threads that hold a row of K logits.
 template <typename T, typename F>
 void with_layout(int64_t K, F&& fn) {
-    if (K <= 8) fn(Narrow<T, 1, 8>{});
-    else if (K <= 64) fn(Narrow<T, 8, 8>{});
-    else if (K <= 512) fn(Narrow<T, 64, 8>{});
-    else if (K <= 2048) fn(Wide<T, 64, 32>{});
-    else if (K <= 8192) fn(Wide<T, 256, 32>{});
-    else if (K <= 32768) fn(Wide<T, 512, 64>{});
-    else if constexpr (sizeof(T) == 2) {
-        if (K <= 65536) fn(Wide<T, 512, 128>{});
-        else if (K <= 131072) fn(Wide<T, 1024, 128>{});
-        else fn(Streamed<T, 1024>{});
+    if (K <= 8) return fn(Narrow<T, 1, 8>{});
+    if (K <= 64) return fn(Narrow<T, 8, 8>{});
+    if (K <= 512) return fn(Wide<T, 16, 32>{});
+    if (K <= 1024) return fn(Wide<T, 32, 32>{});
+    if (K <= 2048) return fn(Wide<T, 64, 32>{});
+    if (K <= 8192) return fn(Wide<T, 256, 32>{});
+    if constexpr (sizeof(T) == 2) {
+        if (K <= 16384) return fn(Wide<T, 256, 64>{});
+        if (K <= Wide<T, 256, 64, 8>::kMost) return fn(Wide<T, 256, 64, 8>{});
+        if (K <= Wide<T, 512, 64, 8>::kMost) return fn(Wide<T, 512, 64, 8>{});
     } else {
-        if (K <= 65536) fn(Wide<T, 1024, 64>{});
-        else fn(Streamed<T, 1024>{});
+        if (K <= Wide<T, 256, 32, 8>::kMost) return fn(Wide<T, 256, 32, 8>{});
+        if (K <= Wide<T, 512, 32, 8>::kMost) return fn(Wide<T, 512, 32, 8>{});
     }
+    fn(Streamed<T, 512>{});
 }
 
 // For one use of a row.
@@ -520,7 +605,6 @@ template <typename T, typename F>
 void with_pass(int64_t K, F&& fn) {
     if (K <= 8) fn(Narrow<T, 1, 8>{});
     else if (K <= 64) fn(Narrow<T, 8, 8>{});
-    else if (K <= 512) fn(Narrow<T, 64, 8>{});
     else if (K <= 2048) fn(Streamed<T, 64>{});
     else fn(Streamed<T, 256>{});
 }
@@ -542,11 +626,14 @@ int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits,
     if (!logits || !actions || !log_probs || !entropy || row_stride < 0) return SWARM_ERR_ARG;
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        with_layout<E>(K, [&](auto layout) {
+        auto run = [&](auto layout) {
             using R = decltype(layout);
             log_probs_kernel<R><<<grid_of<R>(M, 1 << 20), R::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
                 M, K, static_cast<const E*>(logits), row_stride, actions, log_probs, entropy, bad_actions);
-        });
+        };
+        // a row that no workgroup of 256 holds is read once all the same: nothing uses it a second time
+        if (K > 8192) run(Streamed<E, 512>{});
+        else with_layout<E>(K, run);
     });
     return swarm::record_hip_status();
 }
@@ -567,14 +654,14 @@ int32_t swarm_policy_loss_forward(int32_t dtype, int64_t M, int64_t K, const voi
     if (M > 0) {
         const LossArgs p{actions, old_log_probs, ref_log_probs, advantages, mask_u8, denom, clip_lo, clip_hi, kl_coef,
                          entropy_coef};
-        const bool count = d_logits && mask_u8 && !denom && M > kCountHere;
-        if (count) loss_count_kernel<<<1, 1024, 0, st>>>(M, mask_u8, used_denom);
         with_type(dtype, [&](auto e) {
             using E = decltype(e);
             with_layout<E>(K, [&](auto layout) {
                 using R = decltype(layout);
                 blocks = grid_of<R>(M, kMaxBlocks);
-                loss_rows_kernel<R><<<blocks, R::kThreads, 0, st>>>(M, K, static_cast<const E*>(logits), row_stride, p,
+                const bool count = d_logits && mask_u8 && !denom && blocks > kCountHere;
+                if (count) loss_count_kernel<<<1, 1024, 0, st>>>(M, mask_u8, used_denom);
+                loss_rows_kernel<R><<<blocks, R::kThreads, R::lds_bytes(K), st>>>(M, K, static_cast<const E*>(logits), row_stride, p,
                                                                   count ? used_denom : nullptr, row_stats, partials,
                                                                   static_cast<E*>(d_logits), bad_actions);
             });

@@ -52,8 +52,7 @@ __device__ __forceinline__ void store_own(T* p, const Pack<T, N>& v, int skip) {
 // the sum of v over a row's threads, in every one
 template <int GROUP>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    v = lanes_reduce<64>(v, Add{});
     if constexpr (GROUP > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;

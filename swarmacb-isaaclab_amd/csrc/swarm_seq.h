@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/swarmseq.h"
 #include "../../include/swarmstep.h"
 #include "swarm_launch.h"
@@ -64,6 +66,43 @@ struct Pack {
                 w[j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{v[j], j + 1 < N ? v[j + 1 < N ? j + 1 : j] : 0.0f}), T2));
         }
     }
+};
+
+// op over groups of GROUP <= 64 consecutive lanes, in every lane: within 16 by DPP moves, then the 16- and 32-lane
+// swaps, none of which goes through LDS.
+template <int GROUP, typename Op>
+__device__ __forceinline__ float lanes_reduce(float v, Op&& op) {
+    static_assert(GROUP <= 64 && (GROUP & (GROUP - 1)) == 0, "a power of two");
+    auto moved = [&](auto ctrl) {
+        const int w = __builtin_bit_cast(int, v);
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(w, w, decltype(ctrl)::value, 0xf, 0xf, false));
+    };
+    if constexpr (GROUP >= 2) v = op(v, moved(std::integral_constant<int, 0xB1>{}));     // neighbours
+    if constexpr (GROUP >= 4) v = op(v, moved(std::integral_constant<int, 0x4E>{}));     // pairs of a quad
+    if constexpr (GROUP >= 8) v = op(v, moved(std::integral_constant<int, 0x141>{}));    // quads of 8, mirrored
+    if constexpr (GROUP >= 16) v = op(v, moved(std::integral_constant<int, 0x140>{}));   // halves of 16, mirrored
+    if constexpr (GROUP >= 32) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, v);
+        const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        const uint32_t one = r[0], other = r[1];      // __builtin_bit_cast of r[1] itself reads r[0]
+        v = op(__builtin_bit_cast(float, one), __builtin_bit_cast(float, other));
+    }
+    if constexpr (GROUP >= 64) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, v);
+        const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        const uint32_t one = r[0], other = r[1];      // __builtin_bit_cast of r[1] itself reads r[0]
+        v = op(__builtin_bit_cast(float, one), __builtin_bit_cast(float, other));
+    }
+    return v;
+}
+
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
+// the larger one, or a NaN
+struct Maximum {
+    __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); }
 };
 
 // Calls fn with a value of the element type that `dtype` names; false for an unknown dtype.
