@@ -32,6 +32,8 @@ static_assert(kFwdTile % kTile == 0, "the forward pass saves a state at segment 
 constexpr int kQuarters = kThreads / kChannels;   // threads that join one channel's segments
 constexpr int64_t kFill = 512;                 // workgroups that fill the card (two on each of 256 CUs)
 
+constexpr int64_t kLeastTiles = 4;             // of a chunk: reading less than that twice costs a launch more than it saves
+
 template <int VV, int TILE>
 struct Shape {
     static constexpr int V = VV;                       // channels of a group
@@ -85,12 +87,14 @@ struct Rows {
     Pack<T, V> d[DH ? kSteps : 1];
     float keep[kSteps];
 
+    // ALL: no step from t0 on is padding.
+    template <bool ALL>
     __device__ __forceinline__ void load(const ScanArgs& p, const Lane& l, const T* g, const int64_t (&off)[R],
                                          const T* dh, int64_t dt, int64_t t0) {
         const int64_t end = l.len > 0 ? l.len - 1 : 0;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const int64_t t = t0 + s < end ? t0 + s : end;
+            const int64_t t = ALL || t0 + s < end ? t0 + s : end;
             const T* q = g + t * p.gt;
 #pragma unroll
             for (int r = 0; r < R; ++r) x[r][s].load(q + off[r]);
@@ -106,23 +110,30 @@ __device__ __forceinline__ void compose(float& A, float& B, float a, float b) {
     A = a * A;
 }
 
-// The step that every sequence of the workgroup reaches.
+// The step that every sequence of the workgroup reaches, and the one that none passes.
+struct Span {
+    int64_t whole, live;
+};
+
 template <typename R>
-__device__ __forceinline__ int64_t whole_until(const ScanArgs& p, int64_t len, R& red) {
-    if (!p.lengths) return p.steps;
-    const int short_of = __syncthreads_or(len < p.steps);
-    if (!short_of) return p.steps;
-    int64_t* least = reinterpret_cast<int64_t*>(&red);
+__device__ __forceinline__ Span span_of(const ScanArgs& p, int64_t len, R& red) {
+    if (!p.lengths) return {p.steps, p.steps};
+    int64_t(*ends)[2] = reinterpret_cast<int64_t(*)[2]>(&red);
+    Span s{len, len};
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-        const int64_t other = __shfl_xor(len, o);
-        len = other < len ? other : len;
+        const int64_t least = __shfl_xor(s.whole, o), most = __shfl_xor(s.live, o);
+        s.whole = least < s.whole ? least : s.whole;
+        s.live = most > s.live ? most : s.live;
     }
-    if (threadIdx.x % 64 == 0) least[threadIdx.x / 64] = len;
+    if (threadIdx.x % 64 == 0) ends[threadIdx.x / 64][0] = s.whole, ends[threadIdx.x / 64][1] = s.live;
     __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) len = least[w] < len ? least[w] : len;
+    for (int w = 0; w < kThreads / 64; ++w) {
+        s.whole = ends[w][0] < s.whole ? ends[w][0] : s.whole;
+        s.live = ends[w][1] > s.live ? ends[w][1] : s.live;
+    }
     __syncthreads();
-    return len;
+    return s;
 }
 
 // (A, B) of the chunks [from, to) in their order along the walk, by the joining threads of a channel, in every one
@@ -167,7 +178,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void chunk_kernel(ScanArg
     for (int64_t k = 0; k < p.chunk_tiles; ++k) {
         const int64_t t0 = start(k);
         Rows<T, V, S::kSteps, 2, BWD> now;
-        now.load(p, l, g, off, dhp, dt, t0);
+        now.template load<false>(p, l, g, off, dhp, dt, t0);
         float A[V], B[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) A[j] = 1.0f, B[j] = 0.0f;
@@ -228,7 +239,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
     const int64_t first = chunk * p.chunk_tiles;
     const int64_t last = first + p.chunk_tiles < tiles ? first + p.chunk_tiles : tiles;
     const int64_t off[3] = {0, p.U, 2 * p.U};
-    const int64_t whole = whole_until(p, l.len, red);
+    const Span span = span_of(p, l.len, red);
     float carry = c0 ? c0[at] : 0.0f;      // the channel's state before the tile, in every joining thread
     if (chunk > 0) {
         float A, B;
@@ -239,7 +250,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
         constexpr bool ALL = decltype(all)::value;      // no step of the tile is padding
         const int64_t t0 = tile * kFwdTile + seg * S::kSteps;
         Rows<T, V, S::kSteps, 3, false> rows;
-        rows.load(p, l, g, off, g, 0, t0);
+        rows.template load<ALL>(p, l, g, off, g, 0, t0);
         float a[S::kSteps][V], b[S::kSteps][V], A[V], B[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) A[j] = 1.0f, B[j] = 0.0f;
@@ -305,9 +316,24 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
         }
         __syncthreads();
     };
+    // padding of all sequences: the state stands still, and nothing is read
+    auto pass = [&](int64_t tile) {
+        const int64_t t0 = tile * kFwdTile + seg * S::kSteps;
+        T* out = h + (l.i * p.steps + t0) * p.U + l.u;
+        Pack<T, V> none;
+        none.clear();
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s)
+            if (l.exists && t0 + s < p.steps) none.store(out + s * p.U);
+        if (states && quarter == 0 && jl.exists)
+            for (int k = 0; k < kFwdTile / kTile; ++k)
+                if (tile * kFwdTile + k * kTile < p.steps)
+                    states[(jl.i * saved + tile * (kFwdTile / kTile) + k) * p.U + jl.u + ch % V] = carry;
+    };
     for (int64_t tile = first; tile < last; ++tile) {
-        if ((tile + 1) * kFwdTile <= whole) run(tile, std::true_type{});
-        else run(tile, std::false_type{});
+        if ((tile + 1) * kFwdTile <= span.whole) run(tile, std::true_type{});
+        else if (tile * kFwdTile < span.live) run(tile, std::false_type{});
+        else pass(tile);
     }
     if (chunk == p.chunks - 1 && quarter == 0 && jl.exists) c_last[at] = carry;
 }
@@ -333,7 +359,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
     const int64_t chunk_tiles = p.chunk_tiles * (kFwdTile / kTile), first = chunk * chunk_tiles;
     const int64_t last = first + chunk_tiles < tiles ? first + chunk_tiles : tiles;
     const int64_t off[3] = {0, p.U, 2 * p.U};
-    const int64_t whole = whole_until(p, l.len, red);
+    const Span span = span_of(p, l.len, red);
     float carry = d_last ? d_last[at] : 0.0f;     // E behind the tile
     if (chunk < p.chunks - 1) {
         float A, B;
@@ -345,7 +371,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
         const int64_t t0 = tile * kTile + seg * S::kSteps;
         const float start = states[(jl.i * tiles + tile) * p.U + jl.u + ch % V];
         Rows<T, V, S::kSteps, 3, true> rows;
-        rows.load(p, l, g, off, dhp, dt, t0);
+        rows.template load<ALL>(p, l, g, off, dhp, dt, t0);
         {
             float A[V], B[V], G[V];
 #pragma unroll
@@ -454,9 +480,20 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
         }
         __syncthreads();
     };
+    auto pass = [&](int64_t tile) {
+        const int64_t t0 = tile * kTile + seg * S::kSteps;
+        T* out = dg + (l.i * p.steps + t0) * 3 * p.U + l.u;
+        Pack<T, V> none;
+        none.clear();
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s)
+            for (int r = 0; r < 3; ++r)
+                if (l.exists && t0 + s < p.steps) none.store(out + (s * 3 + r) * p.U);
+    };
     for (int64_t tile = last - 1; tile >= first; --tile) {
-        if ((tile + 1) * kTile <= whole) run(tile, std::true_type{});
-        else run(tile, std::false_type{});
+        if ((tile + 1) * kTile <= span.whole) run(tile, std::true_type{});
+        else if (tile * kTile < span.live) run(tile, std::false_type{});
+        else pass(tile);
     }
     if (d_c0 && chunk == 0 && quarter == 0 && jl.exists) d_c0[at] = carry;
 }
@@ -494,7 +531,7 @@ void split(ScanArgs& p) {
     p.blocks = (p.n * p.groups + per_block - 1) / per_block;
     const int64_t tiles = (p.steps + kFwdTile - 1) / kFwdTile;
     int64_t want = p.blocks >= kFill ? 1 : (kFill + p.blocks - 1) / p.blocks;
-    if (want > tiles) want = tiles;
+    if (want > tiles / kLeastTiles) want = tiles / kLeastTiles > 0 ? tiles / kLeastTiles : 1;
     p.chunk_tiles = (tiles + want - 1) / want;
     p.chunks = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
 }

@@ -463,7 +463,7 @@ template <typename R>
 __device__ __forceinline__ void zero_row(typename R::T* out, int lane, int64_t K) {
     constexpr int V = 16 / sizeof(typename R::T);
     Pack<typename R::T> none;
-    for (int j = 0; j < none.kWords; ++j) none.w[j] = 0u;
+    none.clear();
     const int64_t packs = K / V;
     for (int64_t k = lane; k < packs; k += R::kGroup) none.store(out + k * V);
     for (int64_t k = packs * V + lane; k < K; k += R::kGroup) out[k] = (typename R::T)0.0f;

@@ -17,17 +17,16 @@ using f16 = _Float16;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// sigmoid(x) and 1 - sigmoid(x), both to a few units in the last place: e = exp(-x) stays finite (x is
-// held above -87, where the sigmoid is 1e-38) and 1 - s = e s keeps the small side exact.
+// sigmoid(x) and 1 - sigmoid(x), both to a few units in the last place: e = exp(-x) stays finite (held at 2^126,
+// where the sigmoid is 1e-38; a NaN stays one) and 1 - s = e s keeps the small side exact.
 __device__ __forceinline__ void sigmoid_pair(float x, float& s, float& one_minus) {
-    // not fmaxf: a NaN has to stay one
-    const float e = __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * -kLog2e);
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(x * -kLog2e, 126.0f));
     s = __builtin_amdgcn_rcpf(1.0f + e);
     one_minus = e * s;
 }
 
 __device__ __forceinline__ float sigmoid(float x) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f((x < -87.0f ? -87.0f : x) * -kLog2e));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
 }
 
 // N elements at any address, held as words (a 16-bit element in a register of its own would double what a tile
@@ -41,6 +40,10 @@ struct Pack {
     __device__ __forceinline__ void load(const T* __restrict__ p) {
         w[kWords - 1] = 0u;
         __builtin_memcpy(w, p, N * sizeof(T));
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) w[k] = 0u;
     }
     __device__ __forceinline__ void store(T* __restrict__ p) const { __builtin_memcpy(p, w, N * sizeof(T)); }
 
