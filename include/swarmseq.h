@@ -81,11 +81,14 @@ int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, con
                                      const void* d_stream, int64_t ds_row, void* d_x, void* d_weight, float* work,
                                      void* stream);
 
+int64_t swarm_log_probs_workspace(int64_t M, int64_t K);
 /* log_probs[m] = z[m][a_m] - logsumexp(z[m]) and entropy[m] = -sum_k p_k log p_k over M >= 0 rows of K >= 1
  * logits (rows row_stride apart). A logit of -inf is a choice that cannot be taken. An action outside [0, K)
- * gives NaN and sets *bad_actions (device int32, or NULL) to 1. */
+ * gives NaN and sets *bad_actions (device int32, or NULL) to 1. work: swarm_log_probs_workspace(M, K) floats (NULL
+ * where that is 0). */
 int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits, int64_t row_stride,
-                        const int64_t* actions, float* log_probs, float* entropy, int32_t* bad_actions, void* stream);
+                        const int64_t* actions, float* log_probs, float* entropy, float* work, int32_t* bad_actions,
+                        void* stream);
 
 /* The clipped policy loss over the active rows (mask_u8, NULL: all) of M >= 0 rows of K logits:
  *     l = log p(a),  r = exp(l - old),  pg = -min(r A, clamp(r, clip_lo, clip_hi) A)

@@ -85,7 +85,7 @@ TRAIN_EXPORTS = ["swarm_lstm_seq_forward", "swarm_lstm_seq_backward", "swarm_rsa
 # Every symbol include/swarmseq.h declares (sequence-policy operators, same library).
 SEQ_EXPORTS = ["swarm_gated_scan_workspace", "swarm_gated_scan_forward", "swarm_gated_scan_backward",
                "swarm_gated_step", "swarm_residual_norm_workspace", "swarm_residual_norm_forward",
-               "swarm_residual_norm_backward", "swarm_log_probs", "swarm_policy_loss_forward",
+               "swarm_residual_norm_backward", "swarm_log_probs_workspace", "swarm_log_probs", "swarm_policy_loss_forward",
                "swarm_policy_loss_backward"]
 GATED_TILE = 32                      # SWARM_GATED_TILE (include/swarmseq.h)
 POLICY_LOSS_PARTIALS = 2048 * 6      # SWARM_POLICY_LOSS_PARTIALS (include/swarmseq.h)
@@ -283,7 +283,9 @@ def load() -> C.CDLL:
     lib.swarm_residual_norm_backward.restype = i32
     lib.swarm_residual_norm_backward.argtypes = [i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp, vp]
     lib.swarm_log_probs.restype = i32
-    lib.swarm_log_probs.argtypes = [i32, i64, i64, vp, i64] + [vp] * 5
+    lib.swarm_log_probs.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6
+    lib.swarm_log_probs_workspace.restype = i64
+    lib.swarm_log_probs_workspace.argtypes = [i64, i64]
     lib.swarm_policy_loss_forward.restype = i32
     lib.swarm_policy_loss_forward.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6 + [f32] * 4 + [vp] * 8
     lib.swarm_policy_loss_backward.restype = i32

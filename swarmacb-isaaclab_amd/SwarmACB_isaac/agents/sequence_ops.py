@@ -62,6 +62,11 @@ def _check(rc: int, what: str):
         _native.check(rc, what)
 
 
+def _work(words: int, device):
+    """A call's own workspace of that many floats, None for none."""
+    return torch.empty(words, dtype=torch.float32, device=device) if words > 0 else None
+
+
 class _on:
     """torch.cuda.device(t.device) that costs nothing when it is the current device already."""
 
@@ -123,7 +128,7 @@ def _scan_forward(gates, state, keep, lengths, save: bool):
         last = torch.empty(n, U, dtype=torch.float32, device=gates.device)
         tiles = (torch.empty(n, _native.gated_tiles(T), U, dtype=torch.float32, device=gates.device)
                  if save else None)
-        work = _scan_work(lib, n, T, U, gates.device)
+        work = _work(lib.swarm_gated_scan_workspace(n, T, U), gates.device)
         _check(lib.swarm_gated_scan_forward(_DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1),
                                             _p(state), _p(keep), _p(lengths), _p(h), _p(last), _p(tiles), _p(work),
                                             _stream(gates)), "swarm_gated_scan_forward")
@@ -157,17 +162,12 @@ class _GatedScan(torch.autograd.Function):
                 d_h = _rows(d_h)
             if d_last is not None:
                 d_last = d_last.contiguous()
-            work = _scan_work(lib, n, T, U, gates.device)
+            work = _work(lib.swarm_gated_scan_workspace(n, T, U), gates.device)
             _check(lib.swarm_gated_scan_backward(
                 _DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1), _p(keep), _p(lengths),
                 _p(tiles), _p(d_h), d_h.stride(0) if d_h is not None else 0, d_h.stride(1) if d_h is not None else 0,
                 _p(d_last), _p(d_gates), _p(d_state), _p(work), _stream(gates)), "swarm_gated_scan_backward")
         return d_gates, d_state, None, None
-
-
-def _scan_work(lib, n: int, T: int, U: int, device):
-    words = lib.swarm_gated_scan_workspace(n, T, U)
-    return torch.empty(words, dtype=torch.float32, device=device) if words > 0 else None
 
 
 def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, keep: torch.Tensor | None = None,
@@ -316,7 +316,7 @@ class _ResidualNorm(torch.autograd.Function):
             d_w = work = None
             if weight is not None and ctx.needs_input_grad[2]:
                 d_w = torch.empty_like(weight)
-                work = torch.empty(lib.swarm_residual_norm_workspace(rows, D), dtype=torch.float32, device=s.device)
+                work = _work(lib.swarm_residual_norm_workspace(rows, D), s.device)
             _check(lib.swarm_residual_norm_backward(
                 _DTYPES[s.dtype], rows, D, _p(s), s.stride(0), _p(weight), _p(rstd), _p(d_y), d_y.stride(0),
                 _p(d_out), d_out.stride(0) if d_out is not None else 0, _p(d_x), _p(d_w), _p(work), _stream(s)),
@@ -438,8 +438,10 @@ def categorical_log_probs(logits: torch.Tensor, actions: torch.Tensor):
     with _on(z):
         lp = torch.empty(M, dtype=torch.float32, device=z.device)
         ent = torch.empty(M, dtype=torch.float32, device=z.device)
-        _check(_native.load().swarm_log_probs(_DTYPES[z.dtype], M, K, _p(z), z.stride(0), _p(a), _p(lp), _p(ent),
-                                              _p(_bad_action_flag(z.device)), _stream(z)), "swarm_log_probs")
+        lib = _native.load()
+        work = _work(lib.swarm_log_probs_workspace(M, K), z.device)
+        _check(lib.swarm_log_probs(_DTYPES[z.dtype], M, K, _p(z), z.stride(0), _p(a), _p(lp), _p(ent), _p(work),
+                                   _p(_bad_action_flag(z.device)), _stream(z)), "swarm_log_probs")
     return lp.view(actions.shape), ent.view(actions.shape)
 
 

@@ -14,7 +14,7 @@
 // loads are in flight together, and the only serial part is the LDS join. The backward pass reads one saved state
 // per tile and forms the others again, forwards, beside its own backward join.
 //
-// Few channels (one long sequence) do not fill the card: then the length is split into chunks as well, a first
+// Up to kShort steps need no tiles. Few channels (one long sequence) do not fill the card: then the length is split into chunks as well, a first
 // kernel composes each chunk, and the main kernel's workgroups start from the chunks before theirs.
 #include <type_traits>
 
@@ -76,6 +76,11 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& p, int64_t group) {
     if (l.len > p.steps) l.len = p.steps;
     if (l.len < 0) l.len = 0;
     return l;
+}
+
+// what the state is multiplied by before step t
+__device__ __forceinline__ float keep_of(const ScanArgs& p, int64_t i, int64_t t) {
+    return p.keep && t > 0 ? p.keep[i * p.steps + t - 1] : 1.0f;
 }
 
 // A thread's steps of one tile: R of the gate blocks (block r at column off[r]), with DH the gradient of h, and
@@ -498,6 +503,125 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
     if (d_c0 && chunk == 0 && quarter == 0 && jl.exists) d_c0[at] = carry;
 }
 
+// Sequences of at most kShort steps: a thread walks its channels through all of them, with every step's loads in
+// flight at once and nothing to join. (With 4096 channels, 256 sequences and 4 steps in bf16 the tile kernels, most
+// of whose threads then have no step, took 88 + 93 us forward and backward.)
+constexpr int kShort = 16;
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void short_fwd_kernel(ScanArgs p, const float* __restrict__ c0, T* __restrict__ h,
+                                                             float* __restrict__ c_last, float* __restrict__ states) {
+    const Lane l = lane_of<V>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x);
+    if (!l.exists) return;
+    const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
+    const int64_t at = l.i * p.U + l.u;
+    Pack<T, V> xf[kShort], xz[kShort], xo[kShort];
+    float keep[kShort], c[V];
+#pragma unroll
+    for (int t = 0; t < kShort; ++t) {
+        if (t >= p.steps) continue;
+        const int64_t k = t < l.len ? t : (l.len > 0 ? l.len - 1 : 0);
+        const T* q = g + k * p.gt;
+        xf[t].load(q);
+        xz[t].load(q + p.U);
+        xo[t].load(q + 2 * p.U);
+        keep[t] = keep_of(p, l.i, k);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[j] = c0 ? c0[at + j] : 0.0f;
+    if (states)
+#pragma unroll
+        for (int j = 0; j < V; ++j) states[at + j] = c[j];
+    T* out = h + l.i * p.steps * p.U + l.u;
+#pragma unroll
+    for (int t = 0; t < kShort; ++t) {
+        if (t >= p.steps) continue;
+        const bool on = t < l.len;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float f, m;
+            sigmoid_pair(xf[t].get(j), f, m);
+            const float now = f * (c[j] * keep[t]) + m * xz[t].get(j);
+            c[j] = on ? now : c[j];
+            v[j] = on ? sigmoid(xo[t].get(j)) * now : 0.0f;
+        }
+        Pack<T, V> w;
+        w.set(v);
+        w.store(out + t * p.U);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) c_last[at + j] = c[j];
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void short_bwd_kernel(ScanArgs p, const float* __restrict__ states, const T* dh,
+                                                             int64_t dn, int64_t dt,
+                                                             const float* __restrict__ d_last, T* __restrict__ dg,
+                                                             float* __restrict__ d_c0) {
+    const Lane l = lane_of<V>(p, (int64_t)blockIdx.x * kThreads + threadIdx.x);
+    if (!l.exists) return;
+    const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
+    const T* dhp = dh ? dh + l.i * dn + l.u : g;
+    const int64_t at = l.i * p.U + l.u;
+    Pack<T, V> xf[kShort], xz[kShort], xo[kShort], d[kShort];
+    float keep[kShort], pr[kShort][V], c[V], E[V];
+#pragma unroll
+    for (int t = 0; t < kShort; ++t) {
+        if (t >= p.steps) continue;
+        const int64_t k = t < l.len ? t : (l.len > 0 ? l.len - 1 : 0);
+        const T* q = g + k * p.gt;
+        xf[t].load(q);
+        xz[t].load(q + p.U);
+        xo[t].load(q + 2 * p.U);
+        d[t].load(dhp + k * dt);
+        keep[t] = keep_of(p, l.i, k);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        c[j] = states[at + j];
+        E[j] = d_last ? d_last[at + j] : 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < kShort; ++t) {
+        if (t >= p.steps) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float f, m;
+            sigmoid_pair(xf[t].get(j), f, m);
+            pr[t][j] = c[j] * keep[t];
+            c[j] = t < l.len ? f * pr[t][j] + m * xz[t].get(j) : c[j];
+        }
+    }
+    T* out = dg + l.i * p.steps * 3 * p.U + l.u;
+#pragma unroll
+    for (int t = kShort - 1; t >= 0; --t) {
+        if (t >= p.steps) continue;
+        const bool on = t < l.len;
+        float vf[V], vz[V], vo[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float f, m, o, om;
+            sigmoid_pair(xf[t].get(j), f, m);
+            sigmoid_pair(xo[t].get(j), o, om);
+            const float z = xz[t].get(j), od = o * (dh ? d[t].get(j) : 0.0f), D = od + E[j];
+            vf[j] = on ? D * (pr[t][j] - z) * (f * m) : 0.0f;
+            vz[j] = on ? D * m : 0.0f;
+            vo[j] = on ? od * om * (f * pr[t][j] + m * z) : 0.0f;
+            E[j] = on ? f * keep[t] * D : E[j];
+        }
+        Pack<T, V> wf, wz, wo;
+        wf.set(vf), wz.set(vz), wo.set(vo);
+        T* w = out + t * 3 * p.U;
+        wf.store(w);
+        wz.store(w + p.U);
+        wo.store(w + 2 * p.U);
+    }
+    if (d_c0)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d_c0[at + j] = E[j];
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void step_kernel(int64_t rows, int64_t U, const T* __restrict__ gates, int64_t gr,
                                                         const float* c, const float* __restrict__ keep,
@@ -536,6 +660,23 @@ void split(ScanArgs& p) {
     p.chunks = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
 }
 
+// Short sequences: 8 bytes of channels a thread, so that their steps fit its registers.
+template <typename F>
+void with_short(int32_t dtype, int64_t U, F&& fn) {
+    with_type(dtype, [&](auto e) {
+        constexpr int V = 8 / sizeof(e);
+        if (U >= V) fn(e, std::integral_constant<int, V>{});
+        else fn(e, std::integral_constant<int, 1>{});
+    });
+}
+
+// Groups of V channels in each sequence, and the workgroups with a thread for each; false if they are too many.
+bool short_grid(ScanArgs& p, int64_t V) {
+    p.groups = (p.U + V - 1) / V;
+    p.blocks = (p.n * p.groups + kThreads - 1) / kThreads;
+    return p.blocks <= 0x7fffffff;
+}
+
 template <typename F>
 void with_type_and_width(int32_t dtype, int64_t U, F&& fn) {
     with_type(dtype, [&](auto e) {
@@ -563,9 +704,21 @@ int32_t swarm_gated_scan_forward(int32_t dtype, int64_t n, int64_t T, int64_t U,
     if (n == 0) return SWARM_OK;
     if (!gates || !h || !c_last || gates_t < 0 || gates_n < 0) return SWARM_ERR_ARG;
     ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (T <= kShort) {
+        bool fits = false;
+        with_short(dtype, U, [&](auto e, auto v) {
+            using E = decltype(e);
+            constexpr int V = decltype(v)::value;
+            fits = short_grid(p, V);
+            if (fits)
+                short_fwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
+                                                                              tile_states);
+        });
+        return fits ? swarm::record_hip_status() : SWARM_ERR_ARG;
+    }
     split(p);
     if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type_and_width(dtype, U, [&](auto e, auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
@@ -586,14 +739,26 @@ int32_t swarm_gated_scan_backward(int32_t dtype, int64_t n, int64_t T, int64_t U
     if (!gates || !tile_states || !d_gates || gates_t < 0 || gates_n < 0 || d_h_n < 0 || d_h_t < 0)
         return SWARM_ERR_ARG;
     ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int64_t dt = d_h ? d_h_t : gates_t;      // without d_h the loads go to the gates
+    if (T <= kShort) {
+        bool fits = false;
+        with_short(dtype, U, [&](auto e, auto v) {
+            using E = decltype(e);
+            constexpr int V = decltype(v)::value;
+            fits = short_grid(p, V);
+            if (fits)
+                short_bwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(
+                    p, tile_states, static_cast<const E*>(d_h), d_h_n, dt, d_last, static_cast<E*>(d_gates), d_c0);
+        });
+        return fits ? swarm::record_hip_status() : SWARM_ERR_ARG;
+    }
     split(p);
     if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type_and_width(dtype, U, [&](auto e, auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
         const E* dh = static_cast<const E*>(d_h);
-        const int64_t dt = dh ? d_h_t : gates_t;      // without d_h the loads go to the gates
         if (p.chunks > 1)
             chunk_kernel<E, V, true><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, dh, d_h_n, dt);
         scan_bwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, tile_states, dh, d_h_n, dt, d_last,

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kMaxBlocks = 2048;      // SWARM_POLICY_LOSS_PARTIALS = kSums for each
 constexpr int kSums = 6;              // pg, kl, H, outside, pg + kl_coef kl - entropy_coef H, active rows
+constexpr int kFinish = 256;          // threads of the last sums
 constexpr float kBound = 20.0f;       // bound of the log-ratios
 constexpr float kInactive = -1.0f;    // s of a row that takes no part (s >= 1 elsewhere: e = 1 at the maximum)
 constexpr unsigned kCountHere = 256;  // up to this many workgroups, each counts the active rows itself
@@ -67,24 +68,20 @@ __device__ __forceinline__ void group_sums(float& s, float& t, float* red) {
     }
 }
 
-// A row of few logits: E of them in each of LPR lanes, lane after lane.
-template <typename E, int LPR, int N>
-struct Narrow {
+// A row of at most N logits, in one lane.
+template <typename E, int N>
+struct Single {
     using T = E;
-    static constexpr int kGroup = LPR, kThreads = 256;
+    static constexpr int kGroup = 1, kThreads = 256;
     static constexpr bool kHeld = true;
     float z[N];
     static size_t lds_bytes(int64_t) { return 0; }
 
-
-    __device__ __forceinline__ void load(const T* p, int lane, int64_t K) {
+    __device__ __forceinline__ void load(const T* p, int, int64_t K) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int k = lane + i * LPR;
-            z[i] = (float)p[k < (int)K ? k : (int)K - 1];
-        }
+        for (int k = 0; k < N; ++k) z[k] = (float)p[k < (int)K ? k : (int)K - 1];
 #pragma unroll
-        for (int i = 0; i < N; ++i) z[i] = lane + i * LPR < (int)K ? z[i] : -INFINITY;
+        for (int k = 0; k < N; ++k) z[k] = k < (int)K ? z[k] : -INFINITY;
     }
     // f of all values, a few at a time
     template <typename F>
@@ -93,15 +90,13 @@ struct Narrow {
     }
     // out[k] = f(z_k)
     template <typename F>
-    __device__ __forceinline__ void write(T* out, int lane, int64_t K, F&& f) const {
+    __device__ __forceinline__ void write(T* out, int, int64_t K, F&& f) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int k = lane + i * LPR;
-            if (k < (int)K) out[k] = (T)f(z[i]);
-        }
+        for (int k = 0; k < N; ++k)
+            if (k < (int)K) out[k] = (T)f(z[k]);
     }
     // the thread that stores an element
-    static __device__ __forceinline__ int owner(int64_t a) { return (int)a % LPR; }
+    static __device__ __forceinline__ int owner(int64_t) { return 0; }
 };
 
 // Pack i of a thread of a long row: its first column, and how many of its elements belong to the pack before (the
@@ -271,10 +266,19 @@ struct Stats {
     float m, s, log_s, H;
 };
 
+struct Sums {
+    float m, s, t;
+};
+
+__device__ __forceinline__ Stats stats_from(const Sums& a) {
+    const float s = fabsf(a.m) < INFINITY ? a.s : NAN, log_s = logf(s);
+    return {a.m, s, log_s, log_s - a.t * __builtin_amdgcn_rcpf(s) * kLn2};
+}
+
 // Maximum, then both sums. A row that is not held gathers them in one pass: a running maximum rescales the sums when
 // it grows.
 template <typename R>
-__device__ __forceinline__ Stats stats_of(const R& r, int lane, float* red) {
+__device__ __forceinline__ Sums sums_of(const R& r, int lane, float* red) {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     auto largest = [](const auto& v, float m) {
 #pragma unroll
@@ -308,9 +312,12 @@ __device__ __forceinline__ Stats stats_of(const R& r, int lane, float* red) {
         rescale(group_max<R::kGroup>(m, red));
     }
     group_sums<R::kGroup>(s, t, red);
-    if (!(fabsf(m) < INFINITY)) s = NAN;
-    const float log_s = logf(s);
-    return {m, s, log_s, log_s - t * __builtin_amdgcn_rcpf(s) * kLn2};
+    return {m, s, t};
+}
+
+template <typename R>
+__device__ __forceinline__ Stats stats_of(const R& r, int lane, float* red) {
+    return stats_from(sums_of(r, lane, red));
 }
 
 // log p of a logit
@@ -349,6 +356,51 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void log_p
             ent[m] = st.H;
             if (!a.in && bad) atomicOr(bad, 1);
         }
+    }
+}
+
+// Few long rows: each is read by kParts workgroups, whose maxima and sums are joined by a second kernel.
+constexpr int kJoin = 64;
+
+template <typename T>
+__global__ __launch_bounds__(512) void log_probs_part_kernel(int64_t K, const T* __restrict__ logits, int64_t ld,
+                                                             int64_t part, int64_t parts, float* __restrict__ work) {
+    using R = Streamed<T, 512>;
+    __shared__ float red[2 * 512 / 64];
+    const int64_t m = blockIdx.x / parts, p = blockIdx.x - m * parts;
+    const int64_t from = p * part, size = K - from < part ? K - from : part;
+    R r;
+    r.load(logits + m * ld + from, threadIdx.x, size);
+    const Sums a = sums_of(r, threadIdx.x, red);
+    if (threadIdx.x == 0) {
+        float* w = work + (m * parts + p) * 3;
+        w[0] = a.m, w[1] = a.s, w[2] = a.t;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kJoin) void log_probs_join_kernel(int64_t K, const T* __restrict__ logits, int64_t ld,
+                                                               int64_t parts, const float* __restrict__ work,
+                                                               const int64_t* __restrict__ actions,
+                                                               float* __restrict__ logp, float* __restrict__ ent,
+                                                               int32_t* __restrict__ bad) {
+    const int64_t m = blockIdx.x;
+    const float* w = work + m * parts * 3;
+    const Taken a = taken_of(actions, m, logits + m * ld, K);
+    float top = -INFINITY, s = 0.0f, t = 0.0f;
+    for (int64_t p = threadIdx.x; p < parts; p += kJoin) top = Maximum{}(top, w[3 * p]);
+    top = group_max<kJoin>(top, nullptr);
+    for (int64_t p = threadIdx.x; p < parts; p += kJoin) {
+        const float x = exponent(w[3 * p], top), e = exp2_of(x);
+        s += e * w[3 * p + 1];
+        t += e * (w[3 * p + 2] + x * w[3 * p + 1]);
+    }
+    group_sums<kJoin>(s, t, nullptr);
+    const Stats st = stats_from({top, s, t});
+    if (threadIdx.x == 0) {
+        logp[m] = a.in ? log_prob(st, a.z) : NAN;
+        ent[m] = st.H;
+        if (!a.in && bad) atomicOr(bad, 1);
     }
 }
 
@@ -532,13 +584,13 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 256 ? 4 : 0) void loss_
     }
 }
 
-__global__ __launch_bounds__(256) void loss_finish_kernel(int blocks, int64_t M, int has_mask,
+__global__ __launch_bounds__(kFinish) void loss_finish_kernel(int blocks, int64_t M, int has_mask,
                                                           const float* __restrict__ partials,
                                                           const float* __restrict__ denom, float* __restrict__ loss,
                                                           float* __restrict__ terms, float* __restrict__ used_denom) {
-    __shared__ double red[4][kSums];
+    __shared__ double red[kFinish / 64][kSums];
     double s[kSums] = {};
-    for (int b = threadIdx.x; b < blocks; b += 256)
+    for (int b = threadIdx.x; b < blocks; b += kFinish)
         for (int k = 0; k < kSums; ++k) s[k] += (double)partials[b * kSums + k];
     for (int k = 0; k < kSums; ++k) {
 #pragma unroll
@@ -548,7 +600,7 @@ __global__ __launch_bounds__(256) void loss_finish_kernel(int blocks, int64_t M,
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int k = 0; k < kSums; ++k)
-        for (int w = 1; w < 4; ++w) s[k] += red[w][k];
+        for (int w = 1; w < kFinish / 64; ++w) s[k] += red[w][k];
     const float n = has_mask ? (float)s[5] : (float)M;
     const float d = denom ? *denom : at_least_one(n);
     *loss = (float)(s[4] / (double)d);
@@ -583,8 +635,9 @@ __global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
 // The fewest threads that hold a row of K logits.
 template <typename T, typename F>
 void with_layout(int64_t K, F&& fn) {
-    if (K <= 8) return fn(Narrow<T, 1, 8>{});
-    if (K <= 64) return fn(Narrow<T, 8, 8>{});
+    if (K <= 8) return fn(Single<T, 8>{});
+    if (K <= 64) return fn(Wide<T, 4, 16>{});
+    if (K <= 256) return fn(Wide<T, 8, 32>{});
     if (K <= 512) return fn(Wide<T, 16, 32>{});
     if (K <= 1024) return fn(Wide<T, 32, 32>{});
     if (K <= 2048) return fn(Wide<T, 64, 32>{});
@@ -603,10 +656,26 @@ void with_layout(int64_t K, F&& fn) {
 // For one use of a row.
 template <typename T, typename F>
 void with_pass(int64_t K, F&& fn) {
-    if (K <= 8) fn(Narrow<T, 1, 8>{});
-    else if (K <= 64) fn(Narrow<T, 8, 8>{});
+    if (K <= 8) fn(Single<T, 8>{});
+    else if (K <= 64) fn(Streamed<T, 4>{});
+    else if (K <= 512) fn(Streamed<T, 16>{});
     else if (K <= 2048) fn(Streamed<T, 64>{});
     else fn(Streamed<T, 256>{});
+}
+
+// How log_probs splits rows: long ones, when there are fewer than two for each CU, into parts of at least 8192
+// logits (a workgroup's 512 threads with two packs of 16 bits or four of 32 each).
+struct Parts {
+    int64_t part, parts;
+};
+
+Parts parts_of(int64_t M, int64_t K) {
+    constexpr int64_t kLeast = 8192, kFull = 512;
+    if (M < 1 || M >= kFull || K < 2 * kLeast) return {K, 1};
+    int64_t parts = (kFull + M - 1) / M;
+    if (parts > K / kLeast) parts = K / kLeast;
+    const int64_t part = ((K + parts - 1) / parts + 7) / 8 * 8;
+    return {part, (K + part - 1) / part};
 }
 
 template <typename R>
@@ -619,21 +688,38 @@ unsigned grid_of(int64_t M, int64_t most) {
 
 extern "C" {
 
+int64_t swarm_log_probs_workspace(int64_t M, int64_t K) {
+    if (M < 0 || K < 1 || !sane(M, K)) return SWARM_ERR_ARG;
+    const Parts p = parts_of(M, K);
+    return p.parts > 1 ? M * p.parts * 3 : 0;
+}
+
 int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits, int64_t row_stride,
-                        const int64_t* actions, float* log_probs, float* entropy, int32_t* bad_actions, void* stream) {
+                        const int64_t* actions, float* log_probs, float* entropy, float* work, int32_t* bad_actions,
+                        void* stream) {
     if (!known_type(dtype) || M < 0 || K < 1 || !sane(M, K)) return SWARM_ERR_ARG;
     if (M == 0) return SWARM_OK;
     if (!logits || !actions || !log_probs || !entropy || row_stride < 0) return SWARM_ERR_ARG;
+    if (parts_of(M, K).parts > 1 && !work) return SWARM_ERR_ARG;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
         auto run = [&](auto layout) {
             using R = decltype(layout);
-            log_probs_kernel<R><<<grid_of<R>(M, 1 << 20), R::kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            log_probs_kernel<R><<<grid_of<R>(M, 1 << 20), R::kThreads, 0, st>>>(
                 M, K, static_cast<const E*>(logits), row_stride, actions, log_probs, entropy, bad_actions);
         };
-        // a row that no workgroup of 256 holds is read once all the same: nothing uses it a second time
-        if (K > 8192) run(Streamed<E, 512>{});
-        else with_layout<E>(K, run);
+        const Parts p = parts_of(M, K);
+        if (p.parts > 1) {
+            const E* z = static_cast<const E*>(logits);
+            log_probs_part_kernel<E><<<(unsigned)(M * p.parts), 512, 0, st>>>(K, z, row_stride, p.part, p.parts, work);
+            log_probs_join_kernel<E><<<(unsigned)M, kJoin, 0, st>>>(K, z, row_stride, p.parts, work, actions, log_probs,
+                                                                  entropy, bad_actions);
+        } else if (K > 8192) {      // nothing uses the row a second time: no need to hold it
+            run(Streamed<E, 512>{});
+        } else {
+            with_layout<E>(K, run);
+        }
     });
     return swarm::record_hip_status();
 }
@@ -667,7 +753,7 @@ int32_t swarm_policy_loss_forward(int32_t dtype, int64_t M, int64_t K, const voi
             });
         });
     }
-    loss_finish_kernel<<<1, 256, 0, st>>>((int)blocks, M, mask_u8 != nullptr, partials, denom, loss, terms, used_denom);
+    loss_finish_kernel<<<1, kFinish, 0, st>>>((int)blocks, M, mask_u8 != nullptr, partials, denom, loss, terms, used_denom);
     return swarm::record_hip_status();
 }
 

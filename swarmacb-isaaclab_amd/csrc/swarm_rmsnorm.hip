@@ -3,8 +3,8 @@
 //   s = x + r,  rstd = (mean(s^2) + eps)^-1/2,  n = s rstd,  y = n w
 //   d_x = d_r = rstd (w dy - n mean(w dy n)) + d_stream,   d_w = sum over rows of dy n
 //
-// Memory bound: a row is read once, held in registers by as many threads as it needs (a wave up to 2048 elements,
-// else a workgroup), and written once. Packs of 16 bytes at any alignment; the last pack of a row is moved left to
+// Memory bound: a row is read once, held in registers by as many threads as it needs (part of a wave or a wave up to
+// 2048 elements, else a workgroup), and written once. Packs of 16 bytes at any alignment; the last pack of a row is moved left to
 // end with it, so no load crosses the row: the elements it shares with the pack before are left out of the sums and
 // not stored. The backward pass keeps every thread's columns over all rows of its workgroup and adds the weight
 // gradient there; the workgroups' sums are added in a fixed order by a second kernel.
@@ -20,12 +20,12 @@ constexpr int64_t kResident = 256 * 1024;   // threads of the backward pass, at 
 constexpr int kFinish = 1024;               // threads of the weight gradient's last sum
 constexpr int kFinishCols = 32;
 
-// One row's layout: GROUP threads (a wave, or the whole workgroup), EPT elements of each.
+// One row's layout: GROUP threads (part of a wave, a wave, or the whole workgroup), EPT elements of each.
 template <typename T, int GROUP, int EPT>
 struct Row {
     static constexpr int V = 16 / sizeof(T);
     static constexpr int NP = EPT / V;
-    static constexpr int kThreads = GROUP == 64 ? 256 : GROUP;
+    static constexpr int kThreads = GROUP <= 64 ? 256 : GROUP;
     static constexpr int kRows = kThreads / GROUP;     // rows of a workgroup at a time
     static constexpr int kWaves = kThreads / 64;
 
@@ -52,7 +52,7 @@ __device__ __forceinline__ void store_own(T* p, const Pack<T, N>& v, int skip) {
 // the sum of v over a row's threads, in every one
 template <int GROUP>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-    v = lanes_reduce<64>(v, Add{});
+    v = lanes_reduce<(GROUP < 64 ? GROUP : 64)>(v, Add{});
     if constexpr (GROUP > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -297,6 +297,8 @@ struct Plan {
 
 Plan plan_of(int64_t D, int64_t V, bool backward) {
     if (D < V || D > 16384) return {0, 0};
+    if (D <= 32) return {4, 8};
+    if (D <= 128) return {16, 8};
     if (D <= 512) return {64, 8};
     if (D <= 1024) return backward ? Plan{128, 8} : Plan{64, 16};
     if (D <= 2048) return backward ? Plan{256, 8} : Plan{64, 32};
@@ -311,6 +313,8 @@ void with_plan(const Plan& p, F&& fn) {
     auto call = [&](auto g, auto n) {
         if (p.group == g && p.ept == n) fn(g, n);
     };
+    call(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    call(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     call(integral_constant<int, 64>{}, integral_constant<int, 8>{});
     call(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
     if constexpr (BACKWARD) {
@@ -326,7 +330,7 @@ void with_plan(const Plan& p, F&& fn) {
     }
 }
 
-int64_t at_a_time(const Plan& p) { return p.group == 64 ? 4 : 1; }
+int64_t at_a_time(const Plan& p) { return p.group > 0 && p.group <= 64 ? 256 / p.group : 1; }
 
 // Partial sums of the weight gradient: one for each workgroup of the backward pass.
 int64_t partials_of(int64_t rows, const Plan& p) {

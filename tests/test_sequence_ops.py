@@ -207,9 +207,9 @@ def test_c_abi_refusals():
         assert nb(**kw) == -1, kw
     assert lib.swarm_residual_norm_workspace(-1, 4) == -1 and lib.swarm_residual_norm_workspace(4, 0) == -1
     assert lib.swarm_gated_scan_workspace(0, 5, 5) >= 0
-    lp = lambda dt=0, M=1, K=1, z=p, a=p, o=p, e=p, ld=1: lib.swarm_log_probs(dt, M, K, z, ld, a, o, e, None, None)  # noqa: E731
+    lp = lambda dt=0, M=1, K=1, z=p, a=p, o=p, e=p, ld=1: lib.swarm_log_probs(dt, M, K, z, ld, a, o, e, None, None, None)  # noqa: E731
     assert lp(M=0) == 0
-    for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(o=None), dict(e=None), dict(ld=-1)):
+    for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(o=None), dict(e=None), dict(ld=-1), dict(K=40000)):
         assert lp(**kw) == -1, kw
     lf = lambda dt=0, M=1, K=1, z=p, a=p, old=p, adv=p, lo=0.8, hi=1.2, loss=p, terms=p, used=p, st=p, part=p: (  # noqa: E731
         lib.swarm_policy_loss_forward(dt, M, K, z, 1, a, old, None, adv, None, None, lo, hi, 0.0, 0.0, loss, terms,
