@@ -57,6 +57,13 @@ def test_recurrence(n, T, U, keep, lengths, dtype, gpu_device):
     _check_recurrence(*_recurrence_inputs(gpu_device, n, T, U, dtype, keep, lengths, n * 1000 + T))
 
 
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 255, 256, 257, 511, 513])
+def test_recurrence_at_every_border(T, gpu_device):
+    """Around the lengths where the number of tiles, of saved states or of chunks changes, with ragged ends."""
+    for U in (3, 8, 67):
+        _check_recurrence(*_recurrence_inputs(gpu_device, 3, T, U, torch.bfloat16, True, True, T * 7 + U))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_recurrence_of_a_strided_view_without_state(dtype, gpu_device):
     """Rows of a wider, time-major buffer whose start is not aligned; a gradient that is a broadcast view."""
@@ -195,7 +202,8 @@ def test_step_of_nothing(gpu_device):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,D", [(1, 1), (3, 2), (20, 128), (7, 63), (129, 257), (1000, 512), (33, 1001), (5, 4096),
-                                    (64, 5000), (2, 16384), (3, 20011), (2, 70000)])
+                                    (64, 5000), (2, 16384), (3, 20011), (2, 70000),
+                                    (3000, 16), (777, 31), (1030, 33), (515, 128), (300, 129), (9, 2049), (7, 8193)])
 def test_norm(rows, D, dtype, gpu_device):
     g = _gen(gpu_device, rows + D)
     x, r, dy, ds = (torch.randn(rows, D, device=gpu_device, generator=g).to(dtype) for _ in range(4))
@@ -301,6 +309,43 @@ def test_policy_loss(M, K, dtype, gpu_device):
     scale = float(M * min(K, 1024)) if dtype == torch.float16 else 1.0
     _check_loss(z, a, old, adv, ref, mask, None, scale)
     _check_loss(z, a, old, adv, None, None, torch.tensor(3.5, device=gpu_device), scale * 0.75)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [4, 8, 9, 15, 64, 65, 255, 256, 257, 512, 513, 1024, 1025, 2048, 2049, 8192, 8193, 16384,
+                               16385, 32768, 32769, 65536, 65537])
+def test_rows_at_every_border(K, dtype, gpu_device):
+    """Around the row lengths where another layout takes over; the action in the row's first and last places too."""
+    M = 5
+    z, a, old, adv, ref = _loss_inputs(gpu_device, M, K, dtype, K + 1)
+    a[0], a[1], a[2] = K - 1, 0, max(0, K - 3)
+    l = torch.log_softmax(z.float(), 1).gather(1, a[:, None])[:, 0]
+    old, ref = l - 0.07, l + 0.2
+    _check_loss(z, a, old, adv, ref, None, None)
+    _check_loss(z, a, old, adv, ref, torch.tensor([True, False, True, True, True], device=gpu_device), None, 0.5)
+    lp, ent = _ops().categorical_log_probs(z, a)
+    l, le, H, He, _, _ = R.rows_of(z, a)
+    R.check(lp, l, le, "log_probs")
+    R.check(ent, H, He, "entropy")
+
+
+@pytest.mark.parametrize("M,K", [(1, 20000), (3, 33333), (300, 17000)])
+def test_few_long_rows(M, K, gpu_device):
+    """Rows that are read in parts: parts without any choice, a NaN, an infinity and a row with nothing to take."""
+    z, a, *_ = _loss_inputs(gpu_device, M, K, torch.bfloat16, M + 5)
+    z[0, :K // 2] = -float("inf")
+    a[0] = K - 2
+    if M > 2:
+        z[1, K - 1], z[2] = float("nan"), -float("inf")
+    if M > 3:
+        z[3, 5] = float("inf")
+    lp, ent = _ops().categorical_log_probs(z, a)
+    l, le, H, He, _, _ = R.rows_of(z, a)
+    bad = torch.zeros(M, dtype=torch.bool)
+    bad[1:min(M, 4) if M > 3 else min(M, 3)] = M > 1
+    nan = torch.full((M,), float("nan"), dtype=torch.float64)
+    R.check(lp, torch.where(bad, nan, l), le, "log_probs")
+    R.check(ent, torch.where(bad, nan, H), He, "entropy")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
