@@ -296,6 +296,28 @@ def load() -> C.CDLL:
     return lib
 
 
+_seq_ops = None
+
+
+def seq_ops():
+    """The sequence-policy operators as differentiable torch functions (csrc/swarm_torch.cpp), bound to the
+    library that load() returns; raises if either has not been built."""
+    global _seq_ops
+    if _seq_ops is None:
+        load()
+        import torch  # noqa: F401  (the module links against its libraries)
+        try:
+            from . import _seqops
+        except ImportError as e:
+            raise RuntimeError(f"SwarmACB_isaac._seqops cannot be loaded ({e}); build it with "
+                               "`make -C swarmacb-isaaclab_amd/csrc` or __graft_entry__.build()") from e
+        if (_seqops.GATED_TILE, _seqops.POLICY_LOSS_PARTIALS) != (GATED_TILE, POLICY_LOSS_PARTIALS):
+            raise RuntimeError("SwarmACB_isaac._seqops was built from another include/swarmseq.h")
+        _seqops.bind(LIB_PATH)
+        _seq_ops = _seqops
+    return _seq_ops
+
+
 def check(rc: int, what: str):
     if rc != 0:
         lib = load()

@@ -12,15 +12,15 @@ as float32:
 ``categorical_policy_loss``  clipped ratio + KL to a reference + entropy bonus, from logits, with its gradient
 ``categorical_log_probs``    log-probability of the action and entropy per row (rollouts; no autograd)
 
-On the GPU every call runs the HIP kernels of include/swarmseq.h on the current stream of the tensors'
-device, captures into graphs, and waits for nothing; what the kernels do not take raises ValueError. On the
-CPU the same functions run torch operations (float64 too). The forward outputs are not differentiable twice.
+On the GPU every call runs the HIP kernels of include/swarmseq.h (through csrc/swarm_torch.cpp, which holds the
+backward passes) on the current stream of the tensors' device, captures into graphs, and waits for nothing;
+what the kernels do not take raises ValueError, and so does differentiating twice (RuntimeError). On the CPU the
+same functions run torch operations (float64 too).
 """
 
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from ._trainer import _bad_action_flag, check_policy_inputs
@@ -28,60 +28,13 @@ from ._trainer import _bad_action_flag, check_policy_inputs
 __all__ = ["gated_recurrence", "gated_recurrence_step", "residual_rms_norm", "categorical_policy_loss",
            "categorical_log_probs", "check_policy_inputs"]
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # swarm_dtype_t
+_GPU_TYPES = (torch.float32, torch.bfloat16, torch.float16)   # swarm_dtype_t
 RATIO_BOUND = 20.0     # log-ratios are held inside +- this, as in the learned-option trainer's policy loss
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _stream(t: torch.Tensor) -> int:
-    """The current stream of t's device, without building a torch.cuda.Stream (2 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
-def _once(backward):
-    """once_differentiable for a backward whose gradients are new tensors. Its wrapper costs 9 us a call and is
-    only needed where a graph of the gradients is asked for, which is when gradients are recorded in here."""
-    wrapped = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return (wrapped if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-    return run
 
 
 def _flat(t: torch.Tensor, n: int) -> torch.Tensor:
     """t as n contiguous values."""
     return (t if t.dim() == 1 else t.reshape(n)).contiguous()
-
-
-def _check(rc: int, what: str):
-    if rc != 0:
-        _native.check(rc, what)
-
-
-def _work(words: int, device):
-    """A call's own workspace of that many floats, None for none."""
-    return torch.empty(words, dtype=torch.float32, device=device) if words > 0 else None
-
-
-class _on:
-    """torch.cuda.device(t.device) that costs nothing when it is the current device already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -91,7 +44,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _float_type(t: torch.Tensor, what: str):
     if t.is_cuda:
-        if t.dtype not in _DTYPES:
+        if t.dtype not in _GPU_TYPES:
             raise ValueError(f"{what}: float32, bfloat16 or float16 is needed on the GPU, got {t.dtype}")
     elif not t.is_floating_point():
         raise ValueError(f"{what}: a floating type is needed, got {t.dtype}")
@@ -117,58 +70,6 @@ def _no_grad_operand(t, what: str):
 
 
 # -------------------------------------------------------------------------------- gated recurrence
-
-def _scan_forward(gates, state, keep, lengths, save: bool):
-    """(h, last state, tile states or None)"""
-    n, T, U3 = gates.shape
-    U = U3 // 3
-    lib = _native.load()
-    with _on(gates):
-        h = torch.empty(n, T, U, dtype=gates.dtype, device=gates.device)
-        last = torch.empty(n, U, dtype=torch.float32, device=gates.device)
-        tiles = (torch.empty(n, _native.gated_tiles(T), U, dtype=torch.float32, device=gates.device)
-                 if save else None)
-        work = _work(lib.swarm_gated_scan_workspace(n, T, U), gates.device)
-        _check(lib.swarm_gated_scan_forward(_DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1),
-                                            _p(state), _p(keep), _p(lengths), _p(h), _p(last), _p(tiles), _p(work),
-                                            _stream(gates)), "swarm_gated_scan_forward")
-    return h, last, tiles
-
-
-class _GatedScan(torch.autograd.Function):
-    """swarm_gated_scan_forward / _backward. The backward forms the states again from one saved state per
-    tile of steps, so nothing of the size of the sequence is kept but the inputs."""
-
-    @staticmethod
-    def forward(ctx, gates, state, keep, lengths):
-        h, last, tiles = _scan_forward(gates, state, keep, lengths, True)
-        ctx.save_for_backward(gates, keep, lengths, tiles)
-        ctx.has_state = state is not None
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    @_once
-    def backward(ctx, d_h, d_last):
-        gates, keep, lengths, tiles = ctx.saved_tensors
-        n, T, U3 = gates.shape
-        U = U3 // 3
-        lib = _native.load()
-        with _on(gates):
-            d_gates = torch.empty(n, T, U3, dtype=gates.dtype, device=gates.device)
-            d_state = (torch.empty(n, U, dtype=torch.float32, device=gates.device)
-                       if ctx.has_state and ctx.needs_input_grad[1] else None)
-            if d_h is not None:
-                d_h = _rows(d_h)
-            if d_last is not None:
-                d_last = d_last.contiguous()
-            work = _work(lib.swarm_gated_scan_workspace(n, T, U), gates.device)
-            _check(lib.swarm_gated_scan_backward(
-                _DTYPES[gates.dtype], n, T, U, _p(gates), gates.stride(0), gates.stride(1), _p(keep), _p(lengths),
-                _p(tiles), _p(d_h), d_h.stride(0) if d_h is not None else 0, d_h.stride(1) if d_h is not None else 0,
-                _p(d_last), _p(d_gates), _p(d_state), _p(work), _stream(gates)), "swarm_gated_scan_backward")
-        return d_gates, d_state, None, None
-
 
 def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, keep: torch.Tensor | None = None,
                      lengths: torch.Tensor | None = None):
@@ -207,10 +108,7 @@ def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, kee
         lengths = lengths.to(torch.int64).contiguous()
     if state is not None:
         state = state.contiguous()
-    gates = _rows(gates)
-    if torch.is_grad_enabled() and (gates.requires_grad or (state is not None and state.requires_grad)):
-        return _GatedScan.apply(gates, state, keep, lengths)
-    return _scan_forward(gates, state, keep, lengths, False)[:2]
+    return _native.seq_ops().gated_scan(_rows(gates), state, keep, lengths)
 
 
 def _plain_scan(gates, state, keep, lengths):
@@ -265,64 +163,10 @@ def gated_recurrence_step(gates: torch.Tensor, state: torch.Tensor, keep: torch.
     state = state.contiguous()
     if keep is not None:
         keep = keep.to(torch.float32).contiguous()
-    with _on(gates):
-        h = torch.empty(rows, U, dtype=gates.dtype, device=gates.device)
-        out = state if inplace else torch.empty_like(state)
-        _check(_native.load().swarm_gated_step(_DTYPES[gates.dtype], rows, U, _p(gates), gates.stride(0), _p(state),
-                                               _p(keep), _p(h), _p(out), _stream(gates)), "swarm_gated_step")
-    return h, out
+    return _native.seq_ops().gated_step(gates, state, keep, inplace)
 
 
 # ------------------------------------------------------------------------------- residual RMS norm
-
-def _norm_forward(x, residual, weight, eps: float, save: bool):
-    """(y, stream or None, rstd or None)"""
-    rows, D = x.shape
-    with _on(x):
-        y = torch.empty(rows, D, dtype=x.dtype, device=x.device)
-        out = torch.empty_like(y) if residual is not None else None
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if save else None
-        _check(_native.load().swarm_residual_norm_forward(
-            _DTYPES[x.dtype], rows, D, _p(x), x.stride(0), _p(residual),
-            residual.stride(0) if residual is not None else 0, _p(weight), eps, _p(y), _p(out), _p(rstd),
-            _stream(x)), "swarm_residual_norm_forward")
-    return y, out, rstd
-
-
-class _ResidualNorm(torch.autograd.Function):
-    """swarm_residual_norm_forward / _backward over (rows, D); the saved sum is the stream itself."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps: float):
-        y, out, rstd = _norm_forward(x, residual, weight, eps, True)
-        ctx.save_for_backward(out if out is not None else x, weight, rstd)
-        ctx.two = residual is not None
-        ctx.set_materialize_grads(False)
-        return (y, out) if out is not None else y
-
-    @staticmethod
-    @_once
-    def backward(ctx, d_y, d_out=None):
-        s, weight, rstd = ctx.saved_tensors
-        rows, D = s.shape
-        if d_y is None:        # only the stream was used: the sum passes its gradient on
-            return d_out, (d_out if ctx.two else None), (torch.zeros_like(weight) if weight is not None else None), None
-        lib = _native.load()
-        with _on(s):
-            d_y = _rows(d_y)
-            if d_out is not None:
-                d_out = _rows(d_out)
-            d_x = torch.empty(rows, D, dtype=s.dtype, device=s.device)
-            d_w = work = None
-            if weight is not None and ctx.needs_input_grad[2]:
-                d_w = torch.empty_like(weight)
-                work = _work(lib.swarm_residual_norm_workspace(rows, D), s.device)
-            _check(lib.swarm_residual_norm_backward(
-                _DTYPES[s.dtype], rows, D, _p(s), s.stride(0), _p(weight), _p(rstd), _p(d_y), d_y.stride(0),
-                _p(d_out), d_out.stride(0) if d_out is not None else 0, _p(d_x), _p(d_w), _p(work), _stream(s)),
-                "swarm_residual_norm_backward")
-        return d_x, (d_x if ctx.two else None), d_w, None
-
 
 def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None,
                       eps: float = 1e-6):
@@ -349,68 +193,13 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
     x2 = _rows(x if flat else x.reshape(rows, D))
     r2 = None if residual is None else _rows(residual if flat else residual.reshape(rows, D))
     w = None if weight is None else weight.contiguous()
-    if torch.is_grad_enabled() and (x2.requires_grad or (r2 is not None and r2.requires_grad)
-                                    or (w is not None and w.requires_grad)):
-        out = _ResidualNorm.apply(x2, r2, w, float(eps))
-        y, stream = (out, None) if residual is None else out
-    else:
-        y, stream, _ = _norm_forward(x2, r2, w, float(eps), False)
+    y, stream = _native.seq_ops().residual_norm(x2, r2, w, float(eps))
     if residual is None:
         return (y if flat else y.view(x.shape)), x
     return (y, stream) if flat else (y.view(x.shape), stream.view(x.shape))
 
 
 # ------------------------------------------------------------------------------------- policy loss
-
-def _loss_forward(logits, actions, old, adv, ref, mask_u, denom, lo, hi, kl_coef, entropy_coef, save: bool):
-    """(loss, terms, row statistics, denominator, gradient for an incoming gradient of 1 or None)"""
-    M, K = logits.shape
-    dev = logits.device
-    with _on(logits):
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        terms = torch.empty(4, dtype=torch.float32, device=dev)
-        used = torch.empty((), dtype=torch.float32, device=dev)
-        work = torch.empty(_native.POLICY_LOSS_PARTIALS + 4 * M, dtype=torch.float32, device=dev)
-        unit = torch.empty(M, K, dtype=logits.dtype, device=dev) if save and logits.dtype != torch.float16 else None
-        stats = work.data_ptr() + 4 * _native.POLICY_LOSS_PARTIALS
-        _check(_native.load().swarm_policy_loss_forward(
-            _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), _p(old), _p(ref), _p(adv),
-            _p(mask_u), _p(denom), lo, hi, kl_coef, entropy_coef, _p(loss), _p(terms), _p(used), stats, _p(unit),
-            _p(work), _p(_bad_action_flag(dev)), _stream(logits)), "swarm_policy_loss_forward")
-    return loss, terms, work, used, unit
-
-
-class _PolicyLossFromLogits(torch.autograd.Function):
-    """swarm_policy_loss_forward / _backward. The forward call, which has the logits at hand, forms the gradient
-    for an incoming gradient of 1 as well (not in float16, where losses are scaled); the first backward call
-    hands it out, written anew if the incoming gradient is another one, and later calls form their own."""
-
-    @staticmethod
-    def forward(ctx, logits, actions, old, adv, ref, mask_u, denom, lo, hi, kl_coef, entropy_coef):
-        loss, terms, work, used, ctx.unit = _loss_forward(logits, actions, old, adv, ref, mask_u, denom, lo, hi,
-                                                          kl_coef, entropy_coef, True)
-        ctx.save_for_backward(logits, actions, work, used)
-        ctx.entropy_coef = entropy_coef
-        ctx.mark_non_differentiable(terms)
-        return loss, terms
-
-    @staticmethod
-    @_once
-    def backward(ctx, g, _terms):
-        logits, actions, work, used = ctx.saved_tensors
-        M, K = logits.shape
-        d, ctx.unit = ctx.unit, None
-        with _on(logits):
-            have = d is not None
-            if not have:
-                d = torch.empty(M, K, dtype=logits.dtype, device=logits.device)
-            g = g.contiguous()
-            _check(_native.load().swarm_policy_loss_backward(
-                _DTYPES[logits.dtype], M, K, _p(logits), logits.stride(0), _p(actions), ctx.entropy_coef,
-                work.data_ptr() + 4 * _native.POLICY_LOSS_PARTIALS, _p(used), _p(g), have, _p(d), _stream(logits)),
-                "swarm_policy_loss_backward")
-        return (d,) + (None,) * 10
-
 
 def _logit_rows(logits, actions, what: str):
     if not torch.is_tensor(logits) or logits.dim() < 1 or logits.shape[-1] == 0:
@@ -435,13 +224,7 @@ def categorical_log_probs(logits: torch.Tensor, actions: torch.Tensor):
     if not z.is_cuda:
         lp, ent = _plain_log_probs(z, a)
         return lp.reshape(actions.shape), ent.reshape(actions.shape)
-    with _on(z):
-        lp = torch.empty(M, dtype=torch.float32, device=z.device)
-        ent = torch.empty(M, dtype=torch.float32, device=z.device)
-        lib = _native.load()
-        work = _work(lib.swarm_log_probs_workspace(M, K), z.device)
-        _check(lib.swarm_log_probs(_DTYPES[z.dtype], M, K, _p(z), z.stride(0), _p(a), _p(lp), _p(ent), _p(work),
-                                   _p(_bad_action_flag(z.device)), _stream(z)), "swarm_log_probs")
+    lp, ent = _native.seq_ops().log_probs(z, a, _bad_action_flag(z.device))
     return lp.view(actions.shape), ent.view(actions.shape)
 
 
@@ -494,11 +277,8 @@ def categorical_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_log
     d = None if denom is None else denom.reshape(()).contiguous()
     if not z.is_cuda:
         return _plain_policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef))
-    args = (z, a, old, adv, ref, None if active is None else active.view(torch.uint8), d, lo, hi, float(kl_coef),
-            float(entropy_coef))
-    if torch.is_grad_enabled() and z.requires_grad:
-        return _PolicyLossFromLogits.apply(*args)
-    return _loss_forward(*args, False)[:2]
+    return _native.seq_ops().policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef),
+                                         _bad_action_flag(z.device))
 
 
 def _plain_policy_loss(z, a, old, adv, ref, active, denom, lo, hi, kl_coef, entropy_coef):

@@ -565,6 +565,20 @@ def test_together_gradients(gpu_device):
         assert float((a.cpu().double() - b).abs().max()) <= 300 * R.E * float(b.abs().max()), name
 
 
+def test_not_differentiable_twice(gpu_device):
+    """A graph of a gradient can be asked for, but not walked."""
+    ops = _ops()
+    x = torch.randn(4, 5, 24, device=gpu_device, requires_grad=True)
+    w = torch.ones(24, device=gpu_device, requires_grad=True)
+    a = torch.zeros(4, 5, dtype=torch.long, device=gpu_device)
+    f = torch.zeros(4, 5, device=gpu_device)
+    for call in (lambda: ops.gated_recurrence(x)[0].square().sum(), lambda: ops.residual_rms_norm(x, None, w)[0].square().sum(),
+                 lambda: ops.categorical_policy_loss(x, a, f, f)[0]):
+        (d,) = torch.autograd.grad(call(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            d.sum().backward()
+
+
 def test_rollout_equals_sequence(gpu_device):
     """The step form, one decision after another in place, gives the sequence form's outputs."""
     ops = _ops()

@@ -38,6 +38,13 @@ def test_header_constants_agree():
     assert _native.gated_tiles(1) == 1 and _native.gated_tiles(tile) == 1 and _native.gated_tiles(tile + 1) == 2
 
 
+def test_torch_module_binds_the_loaded_library():
+    ops = _native.seq_ops()
+    assert ops is _native.seq_ops() and ops.GATED_TILE == _native.GATED_TILE
+    with pytest.raises(RuntimeError):
+        ops.bind("/nowhere/libswarmstep.so")
+
+
 @pytest.mark.parametrize("n,T,U,with_keep,with_lengths", [(1, 1, 1, False, False), (3, 7, 5, True, False),
                                                           (4, 9, 3, True, True), (2, 6, 4, False, True)])
 def test_recurrence_cpu(n, T, U, with_keep, with_lengths):
