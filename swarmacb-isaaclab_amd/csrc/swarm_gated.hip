@@ -56,6 +56,14 @@ struct ScanArgs {
     float* agg;            // [chunks][2][n][U]: a chunk's A and B
 };
 
+// The workgroup's place. Workgroups go to the eight XCDs in turn; with neighbours on one XCD, neighbouring channels
+// share its L2 and are fetched together (64 x 1024 x 2048, bf16, ragged: forward 217 -> 203 us, backward 380 -> 360).
+// Where the length is split as well that gains nothing (4 x 4096 x 1024, f32: 44 against 47 us forward).
+__device__ __forceinline__ int64_t place_of(const ScanArgs& p) {
+    const unsigned per = gridDim.x / 8, b = blockIdx.x;
+    return p.chunks == 1 && b < per * 8 ? (b % 8) * per + b / 8 : b;
+}
+
 // What a thread works on: V channels of one sequence, from u on. The last group of a sequence starts at U - V, so
 // that no vector load crosses a row's end: it may share channels with the one before, and both write the same.
 // Threads behind the last group read what the last group reads, and write nothing.
@@ -232,7 +240,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
     using S = Shape<V, kFwdTile>;
     __shared__ float ab[2][S::kSegs][kChannels];
     __shared__ __align__(8) float red[kQuarters][kChannels][2];
-    const int64_t chunk = blockIdx.x / p.blocks, block = blockIdx.x - chunk * p.blocks;
+    const int64_t place = place_of(p), chunk = place / p.blocks, block = place - chunk * p.blocks;
     const int lane = threadIdx.x % S::kGroups, seg = threadIdx.x / S::kGroups;
     const Lane l = lane_of<V>(p, block * S::kGroups + lane);
     const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
     __shared__ float ab[3][S::kSegs][kChannels];     // A, B and the gradient's B; then the states before and behind
     __shared__ __align__(8) float red[kQuarters][kChannels][3];
     float (*before)[kChannels][2] = reinterpret_cast<float (*)[kChannels][2]>(&red[0][0][0]);
-    const int64_t chunk = blockIdx.x / p.blocks, block = blockIdx.x - chunk * p.blocks;
+    const int64_t place = place_of(p), chunk = place / p.blocks, block = place - chunk * p.blocks;
     const int lane = threadIdx.x % S::kGroups, seg = threadIdx.x / S::kGroups;
     const Lane l = lane_of<V>(p, block * S::kGroups + lane);
     const T* g = static_cast<const T*>(p.gates) + l.i * p.gn + l.u;
