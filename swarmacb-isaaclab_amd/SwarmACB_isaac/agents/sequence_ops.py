@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _native
-from ._trainer import _bad_action_flag, check_policy_inputs
+from ._trainer import _BAD_ACTIONS, _bad_action_flag, _flag_key, check_policy_inputs
 
 __all__ = ["gated_recurrence", "gated_recurrence_step", "residual_rms_norm", "categorical_policy_loss",
            "categorical_log_probs", "check_policy_inputs"]
@@ -201,6 +201,13 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
 
 # ------------------------------------------------------------------------------------- policy loss
 
+def _flag(device, what: str) -> torch.Tensor:
+    """The device's input-check word. A graph must not be what allocates and clears it."""
+    if _flag_key(device) not in _BAD_ACTIONS and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: run a policy operator on {device} once before capturing one")
+    return _bad_action_flag(device)
+
+
 def _logit_rows(logits, actions, what: str):
     if not torch.is_tensor(logits) or logits.dim() < 1 or logits.shape[-1] == 0:
         raise ValueError(f"{what}: logits (..., K) with K >= 1 are needed")
@@ -224,7 +231,7 @@ def categorical_log_probs(logits: torch.Tensor, actions: torch.Tensor):
     if not z.is_cuda:
         lp, ent = _plain_log_probs(z, a)
         return lp.reshape(actions.shape), ent.reshape(actions.shape)
-    lp, ent = _native.seq_ops().log_probs(z, a, _bad_action_flag(z.device))
+    lp, ent = _native.seq_ops().log_probs(z, a, _flag(z.device, "categorical_log_probs"))
     return lp.view(actions.shape), ent.view(actions.shape)
 
 
@@ -278,7 +285,7 @@ def categorical_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_log
     if not z.is_cuda:
         return _plain_policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef))
     return _native.seq_ops().policy_loss(z, a, old, adv, ref, active, d, lo, hi, float(kl_coef), float(entropy_coef),
-                                         _bad_action_flag(z.device))
+                                         _flag(z.device, what))
 
 
 def _plain_policy_loss(z, a, old, adv, ref, active, denom, lo, hi, kl_coef, entropy_coef):

@@ -646,12 +646,6 @@ __global__ __launch_bounds__(kThreads) void step_kernel(int64_t rows, int64_t U,
     h[id] = (T)(sigmoid((float)g[2 * U]) * now);
 }
 
-bool blocks_of(int64_t items, unsigned& blocks) {
-    const int64_t b = (items + kThreads - 1) / kThreads;
-    blocks = (unsigned)b;
-    return b <= 0x7fffffff;
-}
-
 // Vectors of kWide channels; sequences narrower than that go channel by channel.
 constexpr int kWide = 4;
 int64_t width_of(int64_t U) { return U >= kWide ? kWide : 1; }
@@ -678,11 +672,28 @@ void with_short(int32_t dtype, int64_t U, F&& fn) {
     });
 }
 
-// Groups of V channels in each sequence, and the workgroups with a thread for each; false if they are too many.
-bool short_grid(ScanArgs& p, int64_t V) {
+// Groups of V channels in each sequence, and the workgroups with a thread for each.
+void short_grid(ScanArgs& p, int64_t V) {
     p.groups = (p.U + V - 1) / V;
     p.blocks = (p.n * p.groups + kThreads - 1) / kThreads;
-    return p.blocks <= 0x7fffffff;
+}
+
+// Sequences of a launch: all, unless their threads (four for each channel, at most) pass what a grid counts, and
+// then equal parts, each of which fills the card without its length split. 0: not even one.
+int64_t part_of(int64_t n, int64_t U) {
+    const int64_t most = (kLaunch - kThreads) / (kThreads / kChannels) / ((U + kWide - 1) / kWide * kWide);
+    if (most < 1) return 0;
+    const int64_t parts = (n + most - 1) / most;
+    return (n + parts - 1) / parts;
+}
+
+// p, moved on by elements of a type
+void* ahead(const void* p, int64_t elements, int32_t dtype) {
+    return p ? const_cast<char*>(static_cast<const char*>(p)) + elements * (dtype == SWARM_F32 ? 4 : 2) : nullptr;
+}
+template <typename T>
+T* ahead(T* p, int64_t elements) {
+    return p ? p + elements : nullptr;
 }
 
 template <typename F>
@@ -691,6 +702,61 @@ void with_type_and_width(int32_t dtype, int64_t U, F&& fn) {
         if (width_of(U) == kWide) fn(e, std::integral_constant<int, kWide>{});
         else fn(e, std::integral_constant<int, 1>{});
     });
+}
+
+// One launch's sequences.
+int32_t forward_part(int32_t dtype, const ScanArgs& args, const float* c0, void* h, float* c_last, float* tile_states,
+                     hipStream_t st) {
+    ScanArgs p = args;
+    if (p.steps <= kShort) {
+        with_short(dtype, p.U, [&](auto e, auto v) {
+            using E = decltype(e);
+            constexpr int V = decltype(v)::value;
+            short_grid(p, V);
+            short_fwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
+                                                                          tile_states);
+        });
+        return swarm::record_hip_status();
+    }
+    split(p);
+    if (p.chunks > 1 && !p.agg) return SWARM_ERR_ARG;
+    with_type_and_width(dtype, p.U, [&](auto e, auto v) {
+        using E = decltype(e);
+        constexpr int V = decltype(v)::value;
+        if (p.chunks > 1)
+            chunk_kernel<E, V, false><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, nullptr, 0, 0);
+        scan_fwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
+                                                                                  tile_states);
+    });
+    return swarm::record_hip_status();
+}
+
+int32_t backward_part(int32_t dtype, const ScanArgs& args, const float* tile_states, const void* d_h, int64_t d_h_n,
+                      int64_t d_h_t, const float* d_last, void* d_gates, float* d_c0, hipStream_t st) {
+    ScanArgs p = args;
+    const int64_t dt = d_h ? d_h_t : p.gt;      // without d_h the loads go to the gates
+    if (p.steps <= kShort) {
+        with_short(dtype, p.U, [&](auto e, auto v) {
+            using E = decltype(e);
+            constexpr int V = decltype(v)::value;
+            short_grid(p, V);
+            short_bwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(
+                p, tile_states, static_cast<const E*>(d_h), d_h_n, dt, d_last, static_cast<E*>(d_gates), d_c0);
+        });
+        return swarm::record_hip_status();
+    }
+    split(p);
+    if (p.chunks > 1 && !p.agg) return SWARM_ERR_ARG;
+    with_type_and_width(dtype, p.U, [&](auto e, auto v) {
+        using E = decltype(e);
+        constexpr int V = decltype(v)::value;
+        const E* dh = static_cast<const E*>(d_h);
+        if (p.chunks > 1)
+            chunk_kernel<E, V, true><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, dh, d_h_n, dt);
+        scan_bwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, tile_states, dh, d_h_n, dt, d_last,
+                                                                                  static_cast<E*>(d_gates), d_c0);
+    });
+    return swarm::record_hip_status();
 }
 
 }  // namespace
@@ -710,32 +776,17 @@ int32_t swarm_gated_scan_forward(int32_t dtype, int64_t n, int64_t T, int64_t U,
                                  float* c_last, float* tile_states, float* work, void* stream) {
     if (!known_type(dtype) || n < 0 || T < 1 || U < 1 || !sane(n, T, U)) return SWARM_ERR_ARG;
     if (n == 0) return SWARM_OK;
-    if (!gates || !h || !c_last || gates_t < 0 || gates_n < 0) return SWARM_ERR_ARG;
-    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (T <= kShort) {
-        bool fits = false;
-        with_short(dtype, U, [&](auto e, auto v) {
-            using E = decltype(e);
-            constexpr int V = decltype(v)::value;
-            fits = short_grid(p, V);
-            if (fits)
-                short_fwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
-                                                                              tile_states);
-        });
-        return fits ? swarm::record_hip_status() : SWARM_ERR_ARG;
+    const int64_t part = part_of(n, U);
+    if (!gates || !h || !c_last || gates_t < 0 || gates_n < 0 || part < 1) return SWARM_ERR_ARG;
+    for (int64_t i = 0; i < n; i += part) {
+        const ScanArgs p{n - i < part ? n - i : part, T, U, ahead(gates, i * gates_n, dtype), gates_n, gates_t,
+                         ahead(keep, i * T), ahead(lengths, i), 0, 0, 0, 0, work};
+        const int32_t rc = forward_part(dtype, p, ahead(c0, i * U), ahead(h, i * T * U, dtype), c_last + i * U,
+                                        ahead(tile_states, i * SWARM_GATED_TILES(T) * U),
+                                        static_cast<hipStream_t>(stream));
+        if (rc != SWARM_OK) return rc;
     }
-    split(p);
-    if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
-    with_type_and_width(dtype, U, [&](auto e, auto v) {
-        using E = decltype(e);
-        constexpr int V = decltype(v)::value;
-        if (p.chunks > 1)
-            chunk_kernel<E, V, false><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, nullptr, 0, 0);
-        scan_fwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, c0, static_cast<E*>(h), c_last,
-                                                                                  tile_states);
-    });
-    return swarm::record_hip_status();
+    return SWARM_OK;
 }
 
 int32_t swarm_gated_scan_backward(int32_t dtype, int64_t n, int64_t T, int64_t U, const void* gates, int64_t gates_n,
@@ -744,47 +795,35 @@ int32_t swarm_gated_scan_backward(int32_t dtype, int64_t n, int64_t T, int64_t U
                                   const float* d_last, void* d_gates, float* d_c0, float* work, void* stream) {
     if (!known_type(dtype) || n < 0 || T < 1 || U < 1 || !sane(n, T, U)) return SWARM_ERR_ARG;
     if (n == 0) return SWARM_OK;
-    if (!gates || !tile_states || !d_gates || gates_t < 0 || gates_n < 0 || d_h_n < 0 || d_h_t < 0)
+    const int64_t part = part_of(n, U);
+    if (!gates || !tile_states || !d_gates || gates_t < 0 || gates_n < 0 || d_h_n < 0 || d_h_t < 0 || part < 1)
         return SWARM_ERR_ARG;
-    ScanArgs p{n, T, U, gates, gates_n, gates_t, keep, lengths, 0, 0, 0, 0, work};
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t dt = d_h ? d_h_t : gates_t;      // without d_h the loads go to the gates
-    if (T <= kShort) {
-        bool fits = false;
-        with_short(dtype, U, [&](auto e, auto v) {
-            using E = decltype(e);
-            constexpr int V = decltype(v)::value;
-            fits = short_grid(p, V);
-            if (fits)
-                short_bwd_kernel<E, V><<<(unsigned)p.blocks, kThreads, 0, st>>>(
-                    p, tile_states, static_cast<const E*>(d_h), d_h_n, dt, d_last, static_cast<E*>(d_gates), d_c0);
-        });
-        return fits ? swarm::record_hip_status() : SWARM_ERR_ARG;
+    for (int64_t i = 0; i < n; i += part) {
+        const ScanArgs p{n - i < part ? n - i : part, T, U, ahead(gates, i * gates_n, dtype), gates_n, gates_t,
+                         ahead(keep, i * T), ahead(lengths, i), 0, 0, 0, 0, work};
+        const int32_t rc = backward_part(dtype, p, tile_states + i * SWARM_GATED_TILES(T) * U,
+                                         ahead(d_h, i * d_h_n, dtype), d_h_n, d_h_t, ahead(d_last, i * U),
+                                         ahead(d_gates, i * T * 3 * U, dtype), ahead(d_c0, i * U),
+                                         static_cast<hipStream_t>(stream));
+        if (rc != SWARM_OK) return rc;
     }
-    split(p);
-    if (p.blocks > 0x7fffffff / p.chunks || (p.chunks > 1 && !work)) return SWARM_ERR_ARG;
-    with_type_and_width(dtype, U, [&](auto e, auto v) {
-        using E = decltype(e);
-        constexpr int V = decltype(v)::value;
-        const E* dh = static_cast<const E*>(d_h);
-        if (p.chunks > 1)
-            chunk_kernel<E, V, true><<<(unsigned)(p.blocks * (p.chunks - 1)), kThreads, 0, st>>>(p, dh, d_h_n, dt);
-        scan_bwd_kernel<E, V><<<(unsigned)(p.blocks * p.chunks), kThreads, 0, st>>>(p, tile_states, dh, d_h_n, dt, d_last,
-                                                                                  static_cast<E*>(d_gates), d_c0);
-    });
-    return swarm::record_hip_status();
+    return SWARM_OK;
 }
 
 int32_t swarm_gated_step(int32_t dtype, int64_t rows, int64_t U, const void* gates, int64_t gates_row, const float* c,
                          const float* keep, void* h, float* c_out, void* stream) {
     if (!known_type(dtype) || rows < 0 || U < 1 || !sane(rows, U)) return SWARM_ERR_ARG;
     if (rows == 0) return SWARM_OK;
-    unsigned blocks;
-    if (!gates || !c || !h || !c_out || gates_row < 0 || !blocks_of(rows * U, blocks)) return SWARM_ERR_ARG;
+    const int64_t most = (kLaunch - kThreads) / U;      // rows of a launch
+    if (!gates || !c || !h || !c_out || gates_row < 0 || most < 1) return SWARM_ERR_ARG;
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
-        step_kernel<E><<<blocks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            rows, U, static_cast<const E*>(gates), gates_row, c, keep, static_cast<E*>(h), c_out);
+        for (int64_t r = 0; r < rows; r += most) {
+            const int64_t part = rows - r < most ? rows - r : most;
+            step_kernel<E><<<(unsigned)((part * U + kThreads - 1) / kThreads), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+                part, U, static_cast<const E*>(gates) + r * gates_row, gates_row, c + r * U, ahead(keep, r),
+                static_cast<E*>(h) + r * U, c_out + r * U);
+        }
     });
     return swarm::record_hip_status();
 }

@@ -522,7 +522,7 @@ __device__ __forceinline__ void zero_row(typename R::T* out, int lane, int64_t K
 }
 
 template <typename R>
-__global__ __launch_bounds__(R::kThreads, R::kThreads >= 256 ? 4 : 0) void loss_rows_kernel(
+__global__ __launch_bounds__(R::kThreads, 4) void loss_rows_kernel(
     int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, LossArgs p,
     const float* __restrict__ counted, float* __restrict__ row_stats, float* __restrict__ partials,
     typename R::T* __restrict__ dz, int32_t* __restrict__ bad) {
@@ -632,16 +632,23 @@ __global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
     }
 }
 
-// The fewest threads that hold a row of K logits.
+// The fewest threads that hold a row of K logits; up to kNarrow of them.
+constexpr int64_t kNarrow = 8192;
+
 template <typename T, typename F>
-void with_layout(int64_t K, F&& fn) {
+void with_narrow_layout(int64_t K, F&& fn) {
     if (K <= 8) return fn(Single<T, 8>{});
     if (K <= 64) return fn(Wide<T, 4, 16>{});
     if (K <= 256) return fn(Wide<T, 8, 32>{});
     if (K <= 512) return fn(Wide<T, 16, 32>{});
     if (K <= 1024) return fn(Wide<T, 32, 32>{});
     if (K <= 2048) return fn(Wide<T, 64, 32>{});
-    if (K <= 8192) return fn(Wide<T, 256, 32>{});
+    fn(Wide<T, 256, 32>{});
+}
+
+template <typename T, typename F>
+void with_layout(int64_t K, F&& fn) {
+    if (K <= kNarrow) return with_narrow_layout<T>(K, fn);
     if constexpr (sizeof(T) == 2) {
         if (K <= 16384) return fn(Wide<T, 256, 64>{});
         if (K <= Wide<T, 256, 64, 8>::kMost) return fn(Wide<T, 256, 64, 8>{});
@@ -715,10 +722,10 @@ int32_t swarm_log_probs(int32_t dtype, int64_t M, int64_t K, const void* logits,
             log_probs_part_kernel<E><<<(unsigned)(M * p.parts), 512, 0, st>>>(K, z, row_stride, p.part, p.parts, work);
             log_probs_join_kernel<E><<<(unsigned)M, kJoin, 0, st>>>(K, z, row_stride, p.parts, work, actions, log_probs,
                                                                   entropy, bad_actions);
-        } else if (K > 8192) {      // nothing uses the row a second time: no need to hold it
+        } else if (K > kNarrow) {      // nothing uses the row a second time: no need to hold it
             run(Streamed<E, 512>{});
         } else {
-            with_layout<E>(K, run);
+            with_narrow_layout<E>(K, run);
         }
     });
     return swarm::record_hip_status();

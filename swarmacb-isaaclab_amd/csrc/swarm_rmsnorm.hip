@@ -339,8 +339,6 @@ int64_t partials_of(int64_t rows, const Plan& p) {
     return blocks < most ? blocks : most;
 }
 
-bool fits_grid(int64_t blocks) { return blocks <= 0x7fffffff; }
-
 }  // namespace
 
 extern "C" {
@@ -361,8 +359,7 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
     if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D) || !(eps >= 0.0f)) return SWARM_ERR_ARG;
     if (rows == 0) return SWARM_OK;
     const Plan plan = plan_of(D, dtype == SWARM_F32 ? 4 : 8, false);
-    const int64_t blocks = (rows + at_a_time(plan) - 1) / at_a_time(plan);
-    if (!x || !y || (residual && !stream_out) || x_row < 0 || res_row < 0 || !fits_grid(blocks)) return SWARM_ERR_ARG;
+    if (!x || !y || (residual && !stream_out) || x_row < 0 || res_row < 0) return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     with_type(dtype, [&](auto e) {
         using E = decltype(e);
@@ -376,8 +373,14 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
         }
         with_plan<false>(plan, [&](auto g, auto n) {
             constexpr int G = decltype(g)::value, N = decltype(n)::value;
-            norm_fwd_kernel<E, G, N><<<(unsigned)blocks, Row<E, G, N>::kThreads, 0, st>>>(rows, D, xp, x_row, rp, res_row,
-                                                                                        wp, eps, yp, op, rstd);
+            using R = Row<E, G, N>;
+            constexpr int64_t most = kLaunch / R::kThreads * R::kRows;      // rows of a launch
+            for (int64_t r = 0; r < rows; r += most) {
+                const int64_t part = rows - r < most ? rows - r : most;
+                norm_fwd_kernel<E, G, N><<<(unsigned)((part + R::kRows - 1) / R::kRows), R::kThreads, 0, st>>>(
+                    part, D, xp + r * x_row, x_row, rp ? rp + r * res_row : nullptr, res_row, wp, eps, yp + r * D,
+                    op ? op + r * D : nullptr, rstd ? rstd + r : nullptr);
+            }
         });
     });
     return swarm::record_hip_status();
@@ -389,7 +392,7 @@ int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, con
                                      void* stream) {
     if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D)) return SWARM_ERR_ARG;
     const int64_t cols = (D + kFinishCols - 1) / kFinishCols;
-    if ((d_weight && rows > 0 && !work) || !fits_grid(cols)) return SWARM_ERR_ARG;
+    if (d_weight && ((rows > 0 && !work) || cols > kLaunch / kFinish)) return SWARM_ERR_ARG;
     if (rows == 0 && !d_weight) return SWARM_OK;
     if (rows > 0 && (!sum || !rstd || !d_y || !d_x || sum_row < 0 || dy_row < 0 || ds_row < 0)) return SWARM_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -15,6 +15,8 @@ using f32 = float;
 using bf16 = __bf16;
 using f16 = _Float16;
 
+constexpr int64_t kLaunch = 0xffffffff;      // threads of a launch, at most: a grid's size is counted in threads
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // sigmoid(x) and 1 - sigmoid(x), both to a few units in the last place: e = exp(-x) stays finite (held at 2^126,

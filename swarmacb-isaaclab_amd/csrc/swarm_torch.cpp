@@ -45,6 +45,7 @@ struct Abi {
 #undef X
     const char* (*strerror)(int32_t) = nullptr;
     int32_t (*last_hip_error)() = nullptr;
+    decltype(&hipStreamGetCaptureInfo) capture_info = nullptr;
 };
 Abi abi;
 
@@ -61,6 +62,7 @@ void bind(const std::string& path) {
 #undef X
     abi.strerror = reinterpret_cast<decltype(abi.strerror)>(find("swarm_strerror"));
     abi.last_hip_error = reinterpret_cast<decltype(abi.last_hip_error)>(find("swarm_last_hip_error"));
+    abi.capture_info = reinterpret_cast<decltype(abi.capture_info)>(find("hipStreamGetCaptureInfo"));
 }
 
 void check(int32_t rc, const char* what) {
@@ -79,6 +81,15 @@ int32_t type_of(const Tensor& t) {
 }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// The capture that the stream's calls go into: 0 outside of captures.
+int64_t capture_of(const Tensor& t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (abi.capture_info(c10::hip::getCurrentHIPStream(t.device().index()).stream(), &status, &id) != hipSuccess)
+        throw std::runtime_error("_seqops: the stream's capture is not valid");
+    return status == hipStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id);
+}
 
 template <typename T = void>
 T* ptr(const Tensor& t) {
@@ -280,12 +291,16 @@ Loss loss_forward(const Tensor& logits, const LossArgs& a, bool save) {
 
 // The forward call, which has the logits at hand, forms the gradient for an incoming gradient of 1 as well; the first
 // backward call hands it out, written anew if the incoming gradient is another one, and later calls form their own.
+// So does a backward call captured without its forward call: replays write the buffer again and again.
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     static variable_list forward(AutogradContext* ctx, const Tensor& logits, const LossArgs& a) {
         Loss r = loss_forward(logits, a, true);
         ctx->save_for_backward({logits, a.actions, r.work, r.used});
         ctx->saved_data["entropy_coef"] = a.entropy_coef;
-        if (r.unit.defined()) ctx->saved_data["unit"] = r.unit;
+        if (r.unit.defined()) {
+            ctx->saved_data["unit"] = r.unit;
+            ctx->saved_data["capture"] = capture_of(logits);
+        }
         ctx->mark_non_differentiable({r.terms});
         return {r.loss, r.terms};
     }
@@ -297,13 +312,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const int64_t M = logits.size(0), K = logits.size(1);
         Tensor d;
         const auto unit = ctx->saved_data.find("unit");
-        const bool have = unit != ctx->saved_data.end();
-        if (have) {
-            d = unit->second.toTensor();
-            ctx->saved_data.erase(unit);
-        } else {
-            d = at::empty({M, K}, logits.options());
-        }
+        const bool have = unit != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_of(logits);
+        if (have) d = unit->second.toTensor();
+        else d = at::empty({M, K}, logits.options());
+        if (unit != ctx->saved_data.end()) ctx->saved_data.erase(unit);
         const Tensor g = grads[0].contiguous();
         check(abi.swarm_policy_loss_backward(type_of(logits), M, K, ptr(logits), logits.stride(0), ptr<int64_t>(actions),
                                              static_cast<float>(ctx->saved_data["entropy_coef"].toDouble()),

@@ -175,6 +175,43 @@ def test_recurrence_beyond_32_bits_of_outputs(gpu_device):
         assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -8 * float(b.float().abs().max())
 
 
+@pytest.mark.parametrize("T", [1, 17])
+def test_more_sequences_than_a_grid_counts(T, gpu_device):
+    """More threads than the 2^32 of a launch: sequences at both ends and at the seam equal the same ones alone."""
+    n = 268_435_450
+    gates = torch.empty(n, T, 3, dtype=torch.bfloat16, device=gpu_device).normal_(generator=_gen(gpu_device, 12))
+    d_h = torch.ones((), dtype=torch.bfloat16, device=gpu_device)
+    gates.requires_grad_()
+    h, last = _ops().gated_recurrence(gates)
+    d = torch.autograd.grad(h, gates, d_h.expand(n, T, 1))[0]
+    for part in (slice(0, 9), slice(n // 2 - 9, n // 2 + 9), slice(n - 9, n)):
+        few = gates.detach()[part].clone().requires_grad_()
+        few_h, few_last = _ops().gated_recurrence(few)
+        few_d = torch.autograd.grad(few_h, few, d_h.expand(few.shape[0], T, 1))[0]
+        for a, b in ((h[part], few_h), (last[part], few_last), (d[part], few_d)):
+            # how a length is split may go by the number of channels: a bfloat16 step of the largest values
+            assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -8 * float(b.float().abs().max())
+
+
+def test_more_rows_than_a_grid_counts(gpu_device):
+    """The step form and the norm with more than 2^32 threads: rows at both ends and at the seam equal the same
+    rows alone."""
+    rows, U = (1 << 30) + 5, 4
+    parts = (slice(0, 9), slice((1 << 30) - 100, rows))
+    gates = torch.empty(rows, 3 * U, dtype=torch.bfloat16, device=gpu_device).normal_(generator=_gen(gpu_device, 13))
+    state = torch.ones(rows, U, device=gpu_device)
+    h, c = _ops().gated_recurrence_step(gates, state, inplace=True)
+    for part in parts:
+        few_h, few_c = _ops().gated_recurrence_step(gates[part].clone(), torch.ones_like(c[part]))
+        assert torch.equal(h[part], few_h) and torch.equal(c[part], few_c)
+    del h, c, state, gates
+    x = torch.empty(rows, 8, dtype=torch.bfloat16, device=gpu_device).normal_(generator=_gen(gpu_device, 14))
+    y, stream = _ops().residual_rms_norm(x, x)
+    for part in parts:
+        few_y, few_stream = _ops().residual_rms_norm(x[part].clone(), x[part].clone())
+        assert torch.equal(y[part], few_y) and torch.equal(stream[part], few_stream)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,U", [(1, 1), (20, 64), (333, 67), (4096, 64)])
 def test_step(rows, U, dtype, gpu_device):
@@ -625,6 +662,32 @@ def test_captured_step_replays(U, K, gpu_device):
         got = [t.clone() for t in out]
         for a, b in zip(got, step(dg)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_backward_captured_without_its_forward(dtype, gpu_device):
+    """Every replay of a captured backward call forms the gradient anew, whatever became of the last one."""
+    ops = _ops()
+    z, a, old, adv, ref = _loss_inputs(gpu_device, 30, 900, dtype, 24)
+    ops.categorical_log_probs(z, a)
+    g = torch.ones((), device=gpu_device)
+    side = torch.cuda.Stream(gpu_device)
+    side.wait_stream(torch.cuda.current_stream(gpu_device))
+    with torch.cuda.stream(side):
+        leaf = z.detach().clone().requires_grad_()
+        loss, _ = ops.categorical_policy_loss(leaf, a, old, adv, ref_log_probs=ref, kl_coef=0.1)
+    torch.cuda.synchronize(gpu_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (d,) = torch.autograd.grad(loss, leaf, g, retain_graph=True)
+    with torch.cuda.stream(side):
+        for scale in (1.0, 2.0, 1.0, 1.0, -0.5):
+            g.fill_(scale)
+            d.fill_(7.0)
+            graph.replay()
+            (want,) = torch.autograd.grad(loss, leaf, g, retain_graph=True)
+            side.synchronize()
+            assert torch.equal(d, want)
 
 
 def test_two_streams_at_once(gpu_device):

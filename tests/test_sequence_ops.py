@@ -231,3 +231,16 @@ def test_c_abi_refusals():
     for kw in (dict(dt=7), dict(M=-1), dict(K=0), dict(z=None), dict(a=None), dict(st=None), dict(used=None),
                dict(g=None), dict(d=None)):
         assert lb(**kw) == -1, kw
+
+
+def test_a_graph_does_not_make_the_input_check(monkeypatch):
+    """The word that reports bad actions is made before a capture, or the capture is refused."""
+    from SwarmACB_isaac.agents import _trainer, sequence_ops
+
+    monkeypatch.setattr(_trainer, "_BAD_ACTIONS", {})
+    monkeypatch.setattr(sequence_ops, "_BAD_ACTIONS", _trainer._BAD_ACTIONS)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="once before"):
+        sequence_ops._flag(torch.device("cuda:0"), "categorical_log_probs")
+    flag = _trainer._BAD_ACTIONS["cuda:0"] = torch.zeros(1, dtype=torch.int32)
+    assert sequence_ops._flag(torch.device("cuda:0"), "categorical_log_probs") is flag
