@@ -225,8 +225,96 @@ __global__ __launch_bounds__(kFinish) void weight_finish_kernel(int64_t count, i
     dw[d] = (T)acc;
 }
 
-// Rows narrower than a pack or wider than a workgroup's registers: element by element, the row read again for the
-// second use.
+// Rows narrower than a pack: one thread each. (A workgroup each, as for the widest, took 589 + 876 us for 10^6 rows of
+// 6 in bf16, forward and backward.)
+template <typename T>
+struct NarrowRow {
+    static constexpr int kMost = 16 / sizeof(T) - 1;
+    float v[kMost];
+    __device__ __forceinline__ void load(const T* p, int D) {
+#pragma unroll
+        for (int j = 0; j < kMost; ++j) v[j] = p && j < D ? (float)p[j] : 0.0f;
+    }
+    __device__ __forceinline__ void store(T* p, int D) const {
+#pragma unroll
+        for (int j = 0; j < kMost; ++j)
+            if (j < D) p[j] = (T)v[j];
+    }
+};
+
+constexpr int kNarrow = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kNarrow) void narrow_fwd_kernel(int64_t rows, int D, const T* __restrict__ x, int64_t xr,
+                                                             const T* __restrict__ res, int64_t rr,
+                                                             const T* __restrict__ w, float eps, T* __restrict__ y,
+                                                             T* __restrict__ out, float* __restrict__ rstd) {
+    using R = NarrowRow<T>;
+    R wt;
+    wt.load(w, D);
+    for (int64_t r = (int64_t)blockIdx.x * kNarrow + threadIdx.x; r < rows; r += (int64_t)gridDim.x * kNarrow) {
+        R s, b;
+        s.load(x + r * xr, D);
+        b.load(res ? res + r * rr : nullptr, D);
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < R::kMost; ++j) {
+            s.v[j] += b.v[j];
+            ss += s.v[j] * s.v[j];
+        }
+        const float inv = 1.0f / sqrtf(ss / (float)D + eps);
+        if (res) s.store(out + r * D, D);
+#pragma unroll
+        for (int j = 0; j < R::kMost; ++j) s.v[j] *= inv * (w ? wt.v[j] : 1.0f);
+        s.store(y + r * D, D);
+        if (rstd) rstd[r] = inv;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kNarrow) void narrow_bwd_kernel(int64_t rows, int D, const T* __restrict__ s, int64_t sr,
+                                                             const T* __restrict__ w, const float* __restrict__ rstd,
+                                                             const T* __restrict__ dy, int64_t dyr,
+                                                             const T* __restrict__ ds, int64_t dsr, T* __restrict__ dx,
+                                                             float* __restrict__ partials) {
+    using R = NarrowRow<T>;
+    __shared__ float red[kNarrow / 64][R::kMost];
+    R wt;
+    wt.load(w, D);
+    float dw[R::kMost] = {};
+    for (int64_t r = (int64_t)blockIdx.x * kNarrow + threadIdx.x; r < rows; r += (int64_t)gridDim.x * kNarrow) {
+        const float inv = rstd[r];
+        R n, g, e;
+        n.load(s + r * sr, D);
+        g.load(dy + r * dyr, D);
+        e.load(ds ? ds + r * dsr : nullptr, D);
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < R::kMost; ++j) {
+            n.v[j] *= inv;
+            dw[j] += g.v[j] * n.v[j];
+            g.v[j] *= w ? wt.v[j] : 1.0f;
+            dot += g.v[j] * n.v[j];
+        }
+        const float mean = dot / (float)D;
+#pragma unroll
+        for (int j = 0; j < R::kMost; ++j) e.v[j] += inv * (g.v[j] - n.v[j] * mean);
+        e.store(dx + r * D, D);
+    }
+    if (!partials) return;
+#pragma unroll
+    for (int j = 0; j < R::kMost; ++j) {
+        const float v = lanes_reduce<64>(dw[j], Add{});
+        if (threadIdx.x % 64 == 0) red[threadIdx.x / 64][j] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x >= (unsigned)D) return;
+    float v = 0.0f;
+    for (int k = 0; k < kNarrow / 64; ++k) v += red[k][threadIdx.x];
+    partials[(int64_t)blockIdx.x * D + threadIdx.x] = v;
+}
+
+// Rows wider than a workgroup's registers: element by element, the row read again for the second use.
 constexpr int kPlain = 256;
 
 template <typename T>
@@ -292,11 +380,12 @@ __global__ __launch_bounds__(kPlain) void plain_weight_kernel(int64_t rows, int6
 // barrier. Backward: 8 elements a thread, since a thread also holds the weight and its sums of them; with 16 the
 // kernel took 135 registers, three waves a SIMD, and 123 us where it now takes FIXME (16384 x 4096, bf16).
 struct Plan {
-    int group, ept;      // 0: the plain kernels
+    int group, ept;      // group 1: the narrow kernels, 0: the plain ones
 };
 
 Plan plan_of(int64_t D, int64_t V, bool backward) {
-    if (D < V || D > 16384) return {0, 0};
+    if (D < V) return {1, 0};
+    if (D > 16384) return {0, 0};
     if (D <= 32) return {4, 8};
     if (D <= 128) return {16, 8};
     if (D <= 512) return {64, 8};
@@ -366,6 +455,12 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
         const E *xp = static_cast<const E*>(x), *rp = static_cast<const E*>(residual);
         const E* wp = static_cast<const E*>(weight);
         E *yp = static_cast<E*>(y), *op = static_cast<E*>(stream_out);
+        if (plan.group == 1) {
+            const int64_t blocks = (rows + kNarrow - 1) / kNarrow;
+            narrow_fwd_kernel<E><<<(unsigned)(blocks < 65536 ? blocks : 65536), kNarrow, 0, st>>>(
+                rows, (int)D, xp, x_row, rp, res_row, wp, eps, yp, op, rstd);
+            return;
+        }
         if (plan.group == 0) {
             plain_fwd_kernel<E><<<(unsigned)(rows < 65536 ? rows : 65536), kPlain, 0, st>>>(rows, D, xp, x_row, rp, res_row,
                                                                                         wp, eps, yp, op, rstd);
@@ -404,7 +499,10 @@ int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, con
         const E *yp = static_cast<const E*>(d_y), *dp = static_cast<const E*>(d_stream);
         E* xp = static_cast<E*>(d_x);
         float* partials = d_weight ? work : nullptr;
-        if (rows > 0 && plan.group == 0) {
+        if (rows > 0 && plan.group == 1) {
+            narrow_bwd_kernel<E><<<(unsigned)count, kNarrow, 0, st>>>(rows, (int)D, sp, sum_row, wp, rstd, yp, dy_row, dp,
+                                                                     ds_row, xp, partials);
+        } else if (rows > 0 && plan.group == 0) {
             plain_bwd_kernel<E><<<(unsigned)(rows < 65536 ? rows : 65536), kPlain, 0, st>>>(rows, D, sp, sum_row, wp, rstd,
                                                                                         yp, dy_row, dp, ds_row, xp);
             const int64_t slab = (rows + count - 1) / count;

@@ -263,6 +263,12 @@ def test_norm(rows, D, dtype, gpu_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", [(1, 3), (600, 1), (70001, 5), (300000, 7), (255, 4)])
+def test_norm_of_narrow_rows(rows, D, dtype, gpu_device):
+    test_norm(rows, D, dtype, gpu_device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_norm_of_strided_rows(dtype, gpu_device):
     """Row slices of wider buffers, at offsets that no vector load is aligned to; gradients that are views."""
     rows, D = 37, 200
