@@ -71,13 +71,13 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
                                     void* stream_out, float* rstd, void* stream);
 
 /* d_x = rstd (w d_y - n mean(w d_y n)) + d_stream with n = sum * rstd (the gradient of x and of residual
- * alike), d_weight = column sums of d_y n in a fixed order. sum: the stream_out of the forward pass (x itself
- * without a residual), rows sum_row apart; d_y, d_stream: rows dy_row / ds_row apart, d_stream may be NULL;
- * d_x: [rows][D]; d_weight: [D] of dtype or NULL; work: swarm_residual_norm_workspace(rows, D) floats, needed
- * with d_weight. */
+ * alike), sum = x + residual before any rounding, d_weight = column sums of d_y n in a fixed order. x,
+ * residual, weight: as in the forward pass, which wrote rstd; d_y, d_stream: rows dy_row / ds_row apart,
+ * d_stream may be NULL; d_x: [rows][D]; d_weight: [D] of dtype or NULL; work:
+ * swarm_residual_norm_workspace(rows, D) floats, needed with d_weight. */
 int64_t swarm_residual_norm_workspace(int64_t rows, int64_t D);
-int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, const void* sum, int64_t sum_row,
-                                     const void* weight, const float* rstd, const void* d_y, int64_t dy_row,
+int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, const void* x, int64_t x_row,
+                                     const void* residual, int64_t res_row, const void* weight, const float* rstd, const void* d_y, int64_t dy_row,
                                      const void* d_stream, int64_t ds_row, void* d_x, void* d_weight, float* work,
                                      void* stream);
 

@@ -281,7 +281,7 @@ def load() -> C.CDLL:
     lib.swarm_residual_norm_forward.restype = i32
     lib.swarm_residual_norm_forward.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, f32, vp, vp, vp, vp]
     lib.swarm_residual_norm_backward.restype = i32
-    lib.swarm_residual_norm_backward.argtypes = [i32, i64, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp, vp]
+    lib.swarm_residual_norm_backward.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp, vp]
     lib.swarm_log_probs.restype = i32
     lib.swarm_log_probs.argtypes = [i32, i64, i64, vp, i64] + [vp] * 6
     lib.swarm_log_probs_workspace.restype = i64

@@ -172,8 +172,8 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, wei
                       eps: float = 1e-6):
     """(y, stream): stream = x + residual and y = stream / sqrt(mean(stream^2) + eps) * weight over the last
     dimension; without a residual the stream is x. x and residual (..., D) and weight (D,) share one type;
-    the sum, its norm and y are formed in float32 and rounded once each (y from the sum before its
-    rounding). Gradients flow to all three; the backward reads the stored stream."""
+    the sum, its norm and y are formed in float32 and rounded once each (y, and the gradients, from the sum
+    before its rounding). Gradients flow to all three."""
     if not torch.is_tensor(x) or x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError("residual_rms_norm: x (..., D) with D >= 1 is needed")
     _float_type(x, "residual_rms_norm: x")

@@ -14,6 +14,14 @@
 // of 1 follows at once, from the same registers: reading the logits once and writing their gradient is all the
 // traffic there is. The backward call keeps that gradient if the incoming one is 1, and otherwise forms it again
 // (scaling a rounded gradient would round it twice). Rows that no workgroup holds are read twice.
+//
+// Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
+//   loss, 4096 x 50001, bf16, a tenth masked: 224 us, 3.5 TB/s. Some 115 us of that is arithmetic (two exponentials
+//     an element), and of rows of 100 KB a CU's registers and LDS hold two: too few for one row's loads to hide the
+//     other's arithmetic altogether. Rows read twice took 290 us, three rows a CU of 256 threads each 247 us.
+//   loss, 100000 x 1000, bf16: 95 us, 4.2 TB/s;  20000 x 5000, bf16: 117 us;  4000 x 30000, float32: 218 us, 4.4 TB/s
+//   loss, 2048 x 6, float32: 6.6 + 3.2 us, launches and the last sum
+//   log-probabilities, 8192 x 32768, bf16: 99 us, 5.4 TB/s;  81920 x 18, float32: 3.8 us
 #include <type_traits>
 
 #include "swarm_seq.h"
@@ -339,6 +347,7 @@ __device__ __forceinline__ Taken taken_of(const int64_t* actions, int64_t m, con
     return t;
 }
 
+// Four waves a SIMD: what a row in LDS beside registers, or a long one read in one pass, needs to keep loads in flight.
 template <typename R>
 __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void log_probs_kernel(
     int64_t M, int64_t K, const typename R::T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ actions,
@@ -359,7 +368,7 @@ __global__ __launch_bounds__(R::kThreads, R::kThreads >= 512 ? 4 : 0) void log_p
     }
 }
 
-// Few long rows: each is read by kParts workgroups, whose maxima and sums are joined by a second kernel.
+// Few long rows: each is read by several workgroups, whose maxima and sums are joined by a second kernel.
 constexpr int kJoin = 64;
 
 template <typename T>
@@ -660,7 +669,7 @@ void with_layout(int64_t K, F&& fn) {
     fn(Streamed<T, 512>{});
 }
 
-// For one use of a row.
+// For one use of a row, the backward call's: nothing has to be held.
 template <typename T, typename F>
 void with_pass(int64_t K, F&& fn) {
     if (K <= 8) fn(Single<T, 8>{});
@@ -671,7 +680,7 @@ void with_pass(int64_t K, F&& fn) {
 }
 
 // How log_probs splits rows: long ones, when there are fewer than two for each CU, into parts of at least 8192
-// logits (a workgroup's 512 threads with two packs of 16 bits or four of 32 each).
+// logits (a workgroup's 512 threads with two packs of 16 bits or four of 32 each). 100 x 150000, bf16: 11.6 + 3.8 us.
 struct Parts {
     int64_t part, parts;
 };

@@ -213,13 +213,12 @@ Norm norm_forward(const Tensor& x, const Optional& residual, const Optional& wei
     return r;
 }
 
-// The saved sum is the stream itself.
+// Saved are both addends: the stream that they gave is rounded to its type, and its gradients' sums would show it.
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Optional& residual, const Optional& weight,
                                  double eps) {
         Norm r = norm_forward(x, residual, weight, eps, true);
-        ctx->save_for_backward({residual ? r.stream : x, weight.value_or(Tensor()), r.rstd});
-        ctx->saved_data["two"] = residual.has_value();
+        ctx->save_for_backward({x, residual.value_or(Tensor()), weight.value_or(Tensor()), r.rstd});
         ctx->saved_data["weight"] = wants_grad(weight);
         ctx->set_materialize_grads(false);
         return residual ? variable_list{r.y, r.stream} : variable_list{r.y};
@@ -227,22 +226,23 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &s = saved[0], &weight = saved[1], &rstd = saved[2];
-        const bool two = ctx->saved_data["two"].toBool(), with_w = ctx->saved_data["weight"].toBool();
-        const at::DeviceGuard guard(s.device());
+        const Tensor &x = saved[0], &residual = saved[1], &weight = saved[2], &rstd = saved[3];
+        const bool two = residual.defined(), with_w = ctx->saved_data["weight"].toBool();
+        const at::DeviceGuard guard(x.device());
         const Tensor d_out = two && grads[1].defined() ? rows(grads[1]) : Tensor();
         if (!grads[0].defined())      // only the stream was used: the sum passes its gradient on
             return once({d_out, two ? d_out : Tensor(), with_w ? at::zeros_like(weight) : Tensor(), Tensor()});
-        const int64_t n = s.size(0), D = s.size(1);
-        const Tensor d_y = rows(grads[0]), d_x = at::empty({n, D}, s.options());
+        const int64_t n = x.size(0), D = x.size(1);
+        const Tensor d_y = rows(grads[0]), d_x = at::empty({n, D}, x.options());
         Tensor d_w, work;
         if (with_w) {
-            d_w = at::empty({D}, s.options());
-            work = workspace(s, abi.swarm_residual_norm_workspace(n, D));
+            d_w = at::empty({D}, x.options());
+            work = workspace(x, abi.swarm_residual_norm_workspace(n, D));
         }
-        check(abi.swarm_residual_norm_backward(type_of(s), n, D, ptr(s), s.stride(0), ptr(weight), ptr<float>(rstd),
-                                               ptr(d_y), d_y.stride(0), ptr(d_out), d_out.defined() ? d_out.stride(0) : 0,
-                                               ptr(d_x), ptr(d_w), ptr<float>(work), stream_of(s)),
+        check(abi.swarm_residual_norm_backward(type_of(x), n, D, ptr(x), x.stride(0), ptr(residual),
+                                               two ? residual.stride(0) : 0, ptr(weight), ptr<float>(rstd), ptr(d_y), d_y.stride(0),
+                                               ptr(d_out), d_out.defined() ? d_out.stride(0) : 0, ptr(d_x), ptr(d_w),
+                                               ptr<float>(work), stream_of(x)),
               "swarm_residual_norm_backward");
         return once({d_x, two ? d_x : Tensor(), d_w, Tensor()});
     }

@@ -109,7 +109,7 @@ def norm(x, residual, weight, eps, d_y=None, d_stream=None):
            "stream": (s, rounding(s, dtype) + E * s.abs())}
     if d_y is None:
         return out
-    u = half_step(dtype) if residual is not None else 0.0      # the stored stream's rounding
+    u = E if residual is not None else 0.0      # the sum's rounding
     dy = d_y.double().cpu()
     ds = torch.zeros_like(s) if d_stream is None else d_stream.double().cpu()
     g = dy * w

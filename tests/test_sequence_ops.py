@@ -206,10 +206,10 @@ def test_c_abi_refusals():
     for kw in (dict(dt=4), dict(rows=-1), dict(D=0), dict(x=None), dict(y=None), dict(s=None), dict(eps=-1.0),
                dict(eps=float("nan")), dict(rows=1 << 40, D=1 << 30)):
         assert nf(**kw) == -1, kw
-    nb = lambda dt=0, rows=1, D=1, s=p, rstd=p, dy=p, dx=p, dw=p, work=p: lib.swarm_residual_norm_backward(  # noqa: E731
-        dt, rows, D, s, 1, None, rstd, dy, 1, None, 0, dx, dw, work, None)
+    nb = lambda dt=0, rows=1, D=1, x=p, r=p, rr=1, rstd=p, dy=p, dx=p, dw=p, work=p: lib.swarm_residual_norm_backward(  # noqa: E731
+        dt, rows, D, x, 1, r, rr, None, rstd, dy, 1, None, 0, dx, dw, work, None)
     assert nb(rows=0, dw=None, work=None) == 0
-    for kw in (dict(dt=4), dict(rows=-1), dict(D=0), dict(s=None), dict(rstd=None), dict(dy=None), dict(dx=None),
+    for kw in (dict(dt=4), dict(rows=-1), dict(D=0), dict(x=None), dict(rr=-1), dict(rstd=None), dict(dy=None), dict(dx=None),
                dict(work=None)):
         assert nb(**kw) == -1, kw
     assert lib.swarm_residual_norm_workspace(-1, 4) == -1 and lib.swarm_residual_norm_workspace(4, 0) == -1
