@@ -10,8 +10,10 @@
 // gradient there; the workgroups' sums are added in a fixed order by a second kernel.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
-//   16384 x 4096, bf16: forward 84 us, 6.4 TB/s; backward 109 us, 4.9 TB/s, and 5 us for the weight gradient's last sum
-//   5001 x 1001, float16: 9.2 us, then 14.8 + 6.8 us;  4 000 000 x 16, bf16: 87 and 107 us, 5.9 and 4.8 TB/s
+//   16384 x 4096, bf16: forward 82 us, 6.6 TB/s; backward 139 us, 4.8 TB/s, and 5 us for the weight gradient's last sum
+//   5001 x 1001, float16: 9 us, then 16 + 7 us;  200000 x 512, bf16: 143 and 164 us, 5.7 and 6.2 TB/s
+//   4096 x 16384, float32, where the backward pass spills 80 bytes a thread: 250 and 278 us, 4.3 and 4.8 TB/s
+//   20000 x 20000, bf16, read twice: 1.5 and 2.9 ms, 2.2 and 1.4 TB/s by what one reading would move
 #include <type_traits>
 
 #include "swarm_seq.h"
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(kPlain) void plain_weight_kernel(int64_t rows, int6
 
 // Threads and elements a row takes. Forward: few threads with many loads each, so that rows up to 2048 need no
 // barrier. Backward: 8 elements a thread, since a thread also holds the weight and its sums of them; with 16 the
-// kernel took 135 registers, three waves a SIMD, and 123 us where it now takes 109 (16384 x 4096, bf16).
+// kernel took 135 registers, three waves a SIMD, and 123 us against 109 (16384 x 4096, bf16, without a residual).
 struct Plan {
     int group, ept;      // group 1: the narrow kernels, 0: the plain ones
 };
