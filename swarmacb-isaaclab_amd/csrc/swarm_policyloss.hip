@@ -16,10 +16,11 @@
 // (scaling a rounded gradient would round it twice). Rows that no workgroup holds are read twice.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
-//   loss, 4096 x 50001, bf16, a tenth masked: 224 us, 3.5 TB/s. Some 115 us of that is arithmetic (two exponentials
+//   loss, 4096 x 50001, bf16, a tenth masked: 213 us, 3.6 TB/s. Some 115 us of that is arithmetic (two exponentials
 //     an element), and of rows of 100 KB a CU's registers and LDS hold two: too few for one row's loads to hide the
 //     other's arithmetic altogether. Rows read twice took 290 us, three rows a CU of 256 threads each 247 us.
-//   loss, 100000 x 1000, bf16: 95 us, 4.2 TB/s;  20000 x 5000, bf16: 117 us;  4000 x 30000, float32: 218 us, 4.4 TB/s
+//   loss, 100000 x 1000, bf16: 96 us, 4.2 TB/s;  20000 x 5000, bf16: 102 us, 3.9;  10000 x 15000, bf16: 139 us, 4.3;
+//     10000 x 12000, float32: 218 us, 4.4 TB/s
 //   loss, 2048 x 6, float32: 6.6 + 3.2 us, launches and the last sum
 //   log-probabilities, 8192 x 32768, bf16: 99 us, 5.4 TB/s;  81920 x 18, float32: 3.8 us
 #include <type_traits>
@@ -81,7 +82,6 @@ template <typename E, int N>
 struct Single {
     using T = E;
     static constexpr int kGroup = 1, kThreads = 256;
-    static constexpr bool kHeld = true;
     float z[N];
     static size_t lds_bytes(int64_t) { return 0; }
 
@@ -139,7 +139,6 @@ template <typename E, int GROUP, int EPT, int EXTRA = 0>
 struct Wide {
     using T = E;
     static constexpr int kGroup = GROUP, kThreads = GROUP <= 64 ? 256 : GROUP;
-    static constexpr bool kHeld = true;
     static constexpr int V = 16 / sizeof(T), NP = EPT / V;
     static constexpr int64_t kMost = (int64_t)GROUP * V * (NP + EXTRA);
     Pack<T> x[NP];
@@ -225,7 +224,6 @@ template <typename E, int GROUP>
 struct Streamed {
     using T = E;
     static constexpr int kGroup = GROUP, kThreads = GROUP <= 64 ? 256 : GROUP;
-    static constexpr bool kHeld = false;
     static constexpr int V = 16 / sizeof(T);
     const T* row;
     int64_t K;
@@ -283,8 +281,11 @@ __device__ __forceinline__ Stats stats_from(const Sums& a) {
     return {a.m, s, log_s, log_s - a.t * __builtin_amdgcn_rcpf(s) * kLn2};
 }
 
-// Maximum, then both sums. A row that is not held gathers them in one pass: a running maximum rescales the sums when
-// it grows.
+// Maximum, then both sums. The longest rows (all that are not held, too) gather them in one pass, while their later packs are still on the way: a
+// running maximum rescales the sums when it grows. (4096 x 50001, bf16: 214 us against 224; with 256 threads a row the
+// two passes are even or ahead by up to 2 %.)
+constexpr int kOnePass = 512;
+
 template <typename R>
 __device__ __forceinline__ Sums sums_of(const R& r, int lane, float* red) {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
@@ -301,7 +302,7 @@ __device__ __forceinline__ Sums sums_of(const R& r, int lane, float* red) {
             t += e * x;
         }
     };
-    if constexpr (R::kHeld) {
+    if constexpr (R::kGroup < kOnePass) {
         r.each(lane, [&](const auto& v) { m = largest(v, m); });
         m = group_max<R::kGroup>(m, red);
         r.each(lane, add);
@@ -641,18 +642,35 @@ __global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
     }
 }
 
-// The fewest threads that hold a row of K logits; up to kNarrow of them.
+// Threads that hold a row of K logits, up to kNarrow of them. Few threads with many loads each leave no barrier and
+// little of the last turn unused. 16-bit rows, a thread's 32 / 48 / 64 elements chosen so that few of them are empty,
+// against 32 always (loss, us): 66 logits of 10^6 rows 110 / 145, 300 of 200000 63 / 73, 600 of 150000 90 / 108,
+// 1200 of 80000 93 / 111; above 2048 a wave and two against four waves: 2500 of 40000 109 / 183, 7000 of 15000 102 / 109.
+// For float32 64 elements do not fit the registers, and the same steps gained nothing.
 constexpr int64_t kNarrow = 8192;
 
 template <typename T, typename F>
 void with_narrow_layout(int64_t K, F&& fn) {
     if (K <= 8) return fn(Single<T, 8>{});
     if (K <= 64) return fn(Wide<T, 4, 16>{});
-    if (K <= 256) return fn(Wide<T, 8, 32>{});
-    if (K <= 512) return fn(Wide<T, 16, 32>{});
-    if (K <= 1024) return fn(Wide<T, 32, 32>{});
-    if (K <= 2048) return fn(Wide<T, 64, 32>{});
-    fn(Wide<T, 256, 32>{});
+    if constexpr (sizeof(T) == 2) {
+        if (K <= 128) return fn(Wide<T, 4, 32>{});
+        if (K <= 256) return fn(Wide<T, 8, 32>{});
+        if (K <= 384) return fn(Wide<T, 8, 48>{});
+        if (K <= 512) return fn(Wide<T, 16, 32>{});
+        if (K <= 768) return fn(Wide<T, 16, 48>{});
+        if (K <= 1024) return fn(Wide<T, 32, 32>{});
+        if (K <= 1536) return fn(Wide<T, 32, 48>{});
+        if (K <= 2048) return fn(Wide<T, 64, 32>{});
+        if (K <= 4096) return fn(Wide<T, 64, 64>{});
+        fn(Wide<T, 128, 64>{});
+    } else {
+        if (K <= 256) return fn(Wide<T, 8, 32>{});
+        if (K <= 512) return fn(Wide<T, 16, 32>{});
+        if (K <= 1024) return fn(Wide<T, 32, 32>{});
+        if (K <= 2048) return fn(Wide<T, 64, 32>{});
+        fn(Wide<T, 256, 32>{});
+    }
 }
 
 template <typename T, typename F>

@@ -372,6 +372,12 @@ def test_rows_at_every_border(K, dtype, gpu_device):
     R.check(ent, H, He, "entropy")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [66, 127, 128, 129, 384, 385, 768, 769, 1536, 1537, 2047, 4096, 4097, 8191])
+def test_16_bit_rows_at_every_border(K, dtype, gpu_device):
+    test_rows_at_every_border(K, dtype, gpu_device)
+
+
 @pytest.mark.parametrize("M,K", [(1, 20000), (3, 33333), (300, 17000)])
 def test_few_long_rows(M, K, gpu_device):
     """Rows that are read in parts: parts without any choice, a NaN, an infinity and a row with nothing to take."""
@@ -419,6 +425,11 @@ def test_choices_that_cannot_be_taken(K, dtype, gpu_device):
     assert not lp[16:].any() and not ent[16:].any()
     _, d = _check_loss(z, a, old, adv, ref, None, None, float(M) if dtype == torch.float16 else 1.0)
     assert not d[:, ::2].any() and not d[16:].any()
+
+
+@pytest.mark.parametrize("K", [40000, 50001])
+def test_choices_of_long_rows_that_cannot_be_taken(K, gpu_device):
+    test_choices_that_cannot_be_taken(K, torch.bfloat16, gpu_device)
 
 
 @pytest.mark.parametrize("K", [6, 500, 9000])
@@ -489,6 +500,10 @@ def test_nan_and_infinite_logits_show(K, gpu_device):
     assert loss.isnan() and d[rows].isnan().any(1).all() and d[others].isfinite().all()
     lp, ent = _ops().categorical_log_probs(z, a)
     assert lp[rows].isnan().all() and ent[rows].isnan().all() and lp[others].isfinite().all()
+
+
+def test_nan_and_infinite_logits_show_in_long_rows(gpu_device):
+    test_nan_and_infinite_logits_show(30001, gpu_device)
 
 
 def test_far_log_ratios_are_bounded(gpu_device):
