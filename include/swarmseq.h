@@ -73,13 +73,13 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
 /* d_x = rstd (w d_y - n mean(w d_y n)) + d_stream with n = sum * rstd (the gradient of x and of residual
  * alike), sum = x + residual before any rounding, d_weight = column sums of d_y n in a fixed order. x,
  * residual, weight: as in the forward pass, which wrote rstd; d_y, d_stream: rows dy_row / ds_row apart,
- * d_stream may be NULL; d_x: [rows][D]; d_weight: [D] of dtype or NULL; work:
+ * d_stream may be NULL; d_x: [rows][D]; d_weight: [D <= 2^27 - 32] of dtype or NULL; work:
  * swarm_residual_norm_workspace(rows, D) floats, needed with d_weight. */
 int64_t swarm_residual_norm_workspace(int64_t rows, int64_t D);
 int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, const void* x, int64_t x_row,
-                                     const void* residual, int64_t res_row, const void* weight, const float* rstd, const void* d_y, int64_t dy_row,
-                                     const void* d_stream, int64_t ds_row, void* d_x, void* d_weight, float* work,
-                                     void* stream);
+                                     const void* residual, int64_t res_row, const void* weight, const float* rstd,
+                                     const void* d_y, int64_t dy_row, const void* d_stream, int64_t ds_row, void* d_x,
+                                     void* d_weight, float* work, void* stream);
 
 int64_t swarm_log_probs_workspace(int64_t M, int64_t K);
 /* log_probs[m] = z[m][a_m] - logsumexp(z[m]) and entropy[m] = -sum_k p_k log p_k over M >= 0 rows of K >= 1

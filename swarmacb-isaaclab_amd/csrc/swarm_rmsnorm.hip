@@ -499,9 +499,9 @@ int32_t swarm_residual_norm_forward(int32_t dtype, int64_t rows, int64_t D, cons
 }
 
 int32_t swarm_residual_norm_backward(int32_t dtype, int64_t rows, int64_t D, const void* x, int64_t x_row,
-                                     const void* residual, int64_t res_row, const void* weight, const float* rstd, const void* d_y, int64_t dy_row,
-                                     const void* d_stream, int64_t ds_row, void* d_x, void* d_weight, float* work,
-                                     void* stream) {
+                                     const void* residual, int64_t res_row, const void* weight, const float* rstd,
+                                     const void* d_y, int64_t dy_row, const void* d_stream, int64_t ds_row, void* d_x,
+                                     void* d_weight, float* work, void* stream) {
     if (!known_type(dtype) || rows < 0 || D < 1 || !sane(rows, D)) return SWARM_ERR_ARG;
     const int64_t cols = (D + kFinishCols - 1) / kFinishCols;
     if (d_weight && ((rows > 0 && !work) || cols > kLaunch / kFinish)) return SWARM_ERR_ARG;
