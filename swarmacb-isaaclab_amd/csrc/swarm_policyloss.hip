@@ -281,9 +281,9 @@ __device__ __forceinline__ Stats stats_from(const Sums& a) {
     return {a.m, s, log_s, log_s - a.t * __builtin_amdgcn_rcpf(s) * kLn2};
 }
 
-// Maximum, then both sums. The longest rows (all that are not held, too) gather them in one pass, while their later packs are still on the way: a
-// running maximum rescales the sums when it grows. (4096 x 50001, bf16: 214 us against 224; with 256 threads a row the
-// two passes are even or ahead by up to 2 %.)
+// Maximum, then both sums. The longest rows, and all that are not held, gather them in one pass, while their later
+// packs are still on the way: a running maximum rescales the sums when it grows. (4096 x 50001, bf16: 214 us against
+// 224; with 256 threads a row the two passes are even or ahead by up to 2 %.)
 constexpr int kOnePass = 512;
 
 template <typename R>
