@@ -112,24 +112,31 @@ def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, kee
 
 
 def _plain_scan(gates, state, keep, lengths):
-    n, T, U3 = gates.shape
+    dtype, (n, T, U3) = gates.dtype, gates.shape
     U = U3 // 3
     acc = torch.promote_types(gates.dtype, torch.float32)
-    xf, z, xo = gates.to(acc).split(U, dim=2)
+    gates, before = gates.to(acc), None if keep is None else keep[:, :-1].to(acc)
+    live = None
+    if lengths is not None:
+        # what the padding holds goes before any arithmetic: a selection behind it leaves 0 NaN = NaN to the gradients
+        live = torch.arange(T, device=gates.device)[None] < lengths[:, None]
+        gates = gates.masked_fill(~live[..., None], 0.0)
+        before = None if before is None else before.masked_fill(~live[:, 1:], 1.0)
+    xf, z, xo = gates.split(U, dim=2)
     f, g, o = torch.sigmoid(xf), torch.sigmoid(-xf), torch.sigmoid(xo)
     c = torch.zeros(n, U, dtype=acc, device=gates.device) if state is None else state.to(acc)
     hs = []
     for t in range(T):
-        p = c if keep is None or t == 0 else c * keep[:, t - 1, None].to(acc)
+        p = c if before is None or t == 0 else c * before[:, t - 1, None]
         now = f[:, t] * p + g[:, t] * z[:, t]
         h = o[:, t] * now
-        if lengths is not None:
-            live = (t < lengths)[:, None]
-            now, h = torch.where(live, now, c), torch.where(live, h, torch.zeros_like(h))
+        if live is not None:
+            on = live[:, t, None]
+            now, h = torch.where(on, now, c), torch.where(on, h, torch.zeros_like(h))
         c = now
         hs.append(h)
     h = torch.stack(hs, dim=1) if hs else xf * 0
-    return h.to(gates.dtype), (c.clone() if c is state else c)
+    return h.to(dtype), (c.clone() if c is state else c)
 
 
 def gated_recurrence_step(gates: torch.Tensor, state: torch.Tensor, keep: torch.Tensor | None = None,

@@ -89,6 +89,33 @@ def test_recurrence_of_nothing(T, n):
     assert last.data_ptr() != state.data_ptr() or n == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+@pytest.mark.parametrize("keep_type", [torch.float32, torch.bool, None])
+def test_padding_holds_anything_cpu(keep_type, dtype):
+    """NaN and infinities behind a sequence's end change neither the outputs nor any gradient, which is zero there."""
+    n, T, U = 4, 7, 3
+    lengths = torch.tensor([0, 1, 4, 7])
+    pad = torch.arange(T)[None] >= lengths[:, None]
+    clean, state = _randn(n, T, 3 * U, seed=40).to(dtype).masked_fill(pad[..., None], 0.0), _randn(n, U, seed=41).float()
+    d_h, d_last = _randn(n, T, U, seed=42).to(dtype).masked_fill(pad[..., None], 0.0), _randn(n, U, seed=43)
+    keep = None if keep_type is None else (torch.arange(n * T).view(n, T) % 3 != 1).to(keep_type)
+    out = []
+    for bad in (None, float("nan"), float("inf")):
+        gates, dh, k = clean.clone(), d_h.clone(), None if keep is None else keep.clone()
+        if bad is not None:
+            gates[pad] = dh[pad] = bad
+            if keep_type == torch.float32:
+                k[torch.arange(T)[None] >= lengths[:, None] - 1] = bad      # the last step's has no step behind it
+        gates, s = gates.requires_grad_(), state.clone().requires_grad_()
+        h, last = gated_recurrence(gates, s, k, lengths)
+        out.append((h, last) + torch.autograd.grad((h, last), (gates, s), (dh, d_last.to(last.dtype))))
+    for got in out[1:]:
+        for a, b in zip(got, out[0]):
+            assert a.isfinite().all() and torch.equal(a, b)
+    assert not out[1][0][pad].any() and not out[1][2][pad].any()
+    assert torch.equal(out[1][1][0], state[0].to(out[1][1].dtype))
+
+
 @pytest.mark.parametrize("with_res,with_w", [(True, True), (False, True), (True, False), (False, False)])
 def test_norm_cpu(with_res, with_w):
     x = _randn(3, 2, 7, seed=10).requires_grad_()
