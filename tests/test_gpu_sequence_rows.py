@@ -8,6 +8,8 @@ import sequence_reference as R
 
 pytestmark = pytest.mark.gpu
 
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
 
 def _ops():
     from SwarmACB_isaac.agents import sequence_ops
@@ -116,3 +118,49 @@ def test_masks_are_counted(M, gpu_device):
             n = max(1, int(mask.sum()))
             want = torch.where(mask, (1 - 1 / K) / n, 0.0).double().cpu()
             assert not (d[:, 0].double().cpu() - want).abs().gt(16 * R.E * want).any()
+
+
+# ------------------------------------------------------------------------------------------- the norm
+
+# A workgroup of the backward pass takes these many rows at a time, and a launch has these many workgroups at most.
+def _shape(D, dtype):
+    if D < 16 // dtype.itemsize:
+        return 256, 1024
+    for most, rows, blocks in ((32, 64, 1024), (128, 16, 1024), (512, 4, 1024), (1024, 1, 2048), (2048, 1, 1024),
+                               (4096, 1, 512), (16384, 1, 256)):
+        if D <= most:
+            return rows, blocks
+    return 1, 1024
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D", [(1_000_003, 3), (300_000, 7), (70_001, 5), (140_001, 24), (40_001, 100), (9_001, 300),
+                                    (4_500, 512), (4_301, 1001), (2_100, 2000), (1_501, 4096), (700, 8000), (600, 16384),
+                                    (2_200, 17000)])
+def test_weight_gradient_of_many_rows(rows, D, dtype, gpu_device):
+    """The sum over rows, against the longest chain of additions that it is formed by: a thread's rows, a workgroup's
+    threads, a thirty-second of the workgroups, the last 32. Leaving out one workgroup's rows, or any one of them being
+    counted twice, shows: their share is four times the bound and more."""
+    g = torch.Generator(device=gpu_device).manual_seed(rows + D)
+    x, r, dy, ds = (torch.randn(rows, D, device=gpu_device, generator=g).to(dtype) for _ in range(4))
+    w = (1 + 0.3 * torch.randn(D, device=gpu_device, generator=g)).to(dtype).requires_grad_()
+    xl = x.requires_grad_()
+    y, s = _ops().residual_rms_norm(xl, r, w, eps=1e-5)
+    dx, dw = torch.autograd.grad((y, s), (xl, w), (dy, ds))
+    want = R.norm(x, r, w, 1e-5, dy, ds)
+    R.check(y, *want["y"], "y")
+    R.check(s, *want["stream"], "stream")
+    R.check(dx, *want["dx"], "dx")
+    at_once, most = _shape(D, dtype)
+    count = min(-(-rows // at_once), most)
+    chain = -(-rows // (at_once * count)) + min(at_once, 64) + count / 32 + 32
+    n = x.detach().double().cpu() + r.double().cpu()
+    n = n / torch.sqrt((n * n).mean(1, keepdim=True) + 1e-5)
+    size = (dy.double().cpu() * n).abs().sum(0)
+    value = want["dw"][0]
+    # of every term: the sum's rounding, rstd (half the row sum's error and a few of its own), two products
+    bound = ((D / 64 + 28) + chain) * R.E * size + R.rounding(value, dtype)
+    share = (rows / count) ** 0.5         # of a workgroup's rows, terms of size 1 and either sign
+    accumulated = bound - R.rounding(value, dtype)
+    assert 4 * float(accumulated.max()) < share * (1 if rows > count else 4), "the bound would hide a workgroup"
+    R.check(dw, value, bound, "dw")
