@@ -192,6 +192,9 @@ std::tuple<Tensor, Tensor> gated_step(const Tensor& gates, const Tensor& state, 
     check(abi.swarm_gated_step(type_of(gates), rows, U, ptr(gates), gates.stride(0), ptr<float>(state), ptr<float>(keep),
                                ptr(h), ptr<float>(out), stream_of(gates)),
           "swarm_gated_step");
+    // A backward pass that saved this state has to notice the write. Tensors of inference mode cannot be saved and have
+    // no version.
+    if (inplace && !state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
     return {h, out};
 }
 
