@@ -14,8 +14,8 @@ as float32:
 
 On the GPU every call runs the HIP kernels of include/swarmseq.h (through csrc/swarm_torch.cpp, which holds the
 backward passes) on the current stream of the tensors' device, captures into graphs, and waits for nothing;
-what the kernels do not take raises ValueError, and so does differentiating twice (RuntimeError). On the CPU the
-same functions run torch operations (float64 too).
+what the kernels do not take raises ValueError, dual tensors of forward-mode differentiation included; differentiating
+twice and torch.jit.trace raise RuntimeError. On the CPU the same functions run torch operations (float64 too).
 """
 
 from __future__ import annotations

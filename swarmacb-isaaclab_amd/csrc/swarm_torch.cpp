@@ -7,9 +7,11 @@
 //
 // The C ABI is looked up in the library that the package has loaded (bind()), not linked, so that both always use
 // one and the same build.
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -111,6 +113,19 @@ Tensor workspace(const Tensor& like, int64_t words) {
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Optional& t) { return t && wants_grad(*t); }
 
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const Optional& t) { return t && has_tangent(*t); }
+
+// Kernels write new tensors through their pointers, of which neither forward-mode differentiation nor a trace knows: the
+// one would lose the derivative, the other would record an empty tensor.
+template <typename... Ts>
+void check_recorders(const char* what, const Ts&... operands) {
+    if (torch::jit::tracer::isTracing())
+        throw std::runtime_error(std::string(what) + " cannot be recorded by torch.jit.trace on the GPU");
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && (has_tangent(operands) || ...))
+        throw std::invalid_argument(std::string(what) + " has no forward-mode derivative on the GPU: detach the dual tensor");
+}
+
 // t with its last dimension contiguous
 Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
@@ -177,6 +192,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& gates, const Optional& state, const Optional& keep,
                                       const Optional& lengths) {
+    check_recorders("gated_recurrence", gates, state, keep);
     if (at::GradMode::is_enabled() && (wants_grad(gates) || wants_grad(state))) {
         const auto r = GatedScan::apply(gates, state, keep, lengths);
         return {r[0], r[1]};
@@ -186,6 +202,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& gates, const Optional& state
 }
 
 std::tuple<Tensor, Tensor> gated_step(const Tensor& gates, const Tensor& state, const Optional& keep, bool inplace) {
+    check_recorders("gated_recurrence_step", gates, state, keep);
     const at::DeviceGuard guard(gates.device());
     const int64_t rows = gates.size(0), U = gates.size(1) / 3;
     const Tensor h = at::empty({rows, U}, gates.options()), out = inplace ? state : at::empty_like(state);
@@ -252,6 +269,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 };
 
 std::tuple<Tensor, Optional> residual_norm(const Tensor& x, const Optional& residual, const Optional& weight, double eps) {
+    check_recorders("residual_rms_norm", x, residual, weight);
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual) || wants_grad(weight))) {
         const auto r = ResidualNorm::apply(x, residual, weight, eps);
         return {r[0], residual ? Optional(r[1]) : std::nullopt};
@@ -332,6 +350,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& actions, const Tensor& old_lp, const Tensor& adv,
                                        const Optional& ref, const Optional& mask, const Optional& denom, double lo,
                                        double hi, double kl_coef, double entropy_coef, const Tensor& flag) {
+    check_recorders("categorical_policy_loss", logits, old_lp, adv, ref, denom);
     const LossArgs a{actions, old_lp, adv, ref, mask, denom, lo, hi, kl_coef, entropy_coef, flag};
     if (at::GradMode::is_enabled() && wants_grad(logits)) {
         const auto r = PolicyLoss::apply(logits, a);
@@ -342,6 +361,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& actio
 }
 
 std::tuple<Tensor, Tensor> log_probs(const Tensor& logits, const Tensor& actions, const Tensor& flag) {
+    check_recorders("categorical_log_probs", logits);
     const at::DeviceGuard guard(logits.device());
     const int64_t M = logits.size(0), K = logits.size(1);
     const Tensor lp = floats(logits, {M}), ent = floats(logits, {M});
