@@ -216,9 +216,9 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void chunk_kernel(ScanArg
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 float f, m;
-                sigmoid_pair(now.x[0][s].get(j), f, m);
+                sigmoid_pair<T>(now.x[0][s].get(j), f, m);
                 const float y = now.x[1][s].get(j), a = f * now.keep[s];
-                const float b = BWD ? a * (sigmoid(y) * (has_dh ? now.d[s].get(j) : 0.0f)) : m * y;
+                const float b = BWD ? a * (sigmoid<T>(y) * (has_dh ? now.d[s].get(j) : 0.0f)) : m * y;
                 compose(A[j], B[j], on ? a : 1.0f, on ? b : 0.0f);
             }
         }
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 float f, m;
-                sigmoid_pair(rows.x[0][s].get(j), f, m);
+                sigmoid_pair<T>(rows.x[0][s].get(j), f, m);
                 a[s][j] = on ? f * rows.keep[s] : 1.0f;
                 b[s][j] = on ? m * rows.x[1][s].get(j) : 0.0f;
                 compose(A[j], B[j], a[s][j], b[s][j]);
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_fwd_kernel(Scan
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 now[j] = a[s][j] * now[j] + b[s][j];
-                v[j] = on ? sigmoid(rows.x[2][s].get(j)) * now[j] : 0.0f;
+                v[j] = on ? sigmoid<T>(rows.x[2][s].get(j)) * now[j] : 0.0f;
             }
             Pack<T, V> w;
             w.set(v);
@@ -409,9 +409,9 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float f, m;
-                    sigmoid_pair(rows.x[0][s].get(j), f, m);
+                    sigmoid_pair<T>(rows.x[0][s].get(j), f, m);
                     const float a = on ? f * rows.keep[s] : 1.0f;
-                    const float od = sigmoid(rows.x[2][s].get(j)) * (dh ? rows.d[s].get(j) : 0.0f);
+                    const float od = sigmoid<T>(rows.x[2][s].get(j)) * (dh ? rows.d[s].get(j) : 0.0f);
                     B[j] = a * B[j] + (on ? m * rows.x[1][s].get(j) : 0.0f);
                     A[j] *= a;
                     // E at the segment's first step is the sum of a_0 .. a_s (o dh)_s
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 float f, m;
-                sigmoid_pair(rows.x[0][s].get(j), f, m);
+                sigmoid_pair<T>(rows.x[0][s].get(j), f, m);
                 cs[s][j] = now[j] * rows.keep[s];
                 now[j] = on ? f * cs[s][j] + m * rows.x[1][s].get(j) : now[j];
             }
@@ -485,8 +485,8 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 float f, m, o, om;
-                sigmoid_pair(rows.x[0][s].get(j), f, m);
-                sigmoid_pair(rows.x[2][s].get(j), o, om);
+                sigmoid_pair<T>(rows.x[0][s].get(j), f, m);
+                sigmoid_pair<T>(rows.x[2][s].get(j), o, om);
                 const float z = rows.x[1][s].get(j), pr = cs[s][j];
                 const float cc = f * pr + m * z;
                 const float od = o * (dh ? rows.d[s].get(j) : 0.0f);
@@ -563,10 +563,10 @@ __global__ __launch_bounds__(kThreads) void short_fwd_kernel(ScanArgs p, const f
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float f, m;
-            sigmoid_pair(xf[t].get(j), f, m);
+            sigmoid_pair<T>(xf[t].get(j), f, m);
             const float now = f * (c[j] * keep[t]) + m * xz[t].get(j);
             c[j] = on ? now : c[j];
-            v[j] = on ? sigmoid(xo[t].get(j)) * now : 0.0f;
+            v[j] = on ? sigmoid<T>(xo[t].get(j)) * now : 0.0f;
         }
         Pack<T, V> w;
         w.set(v);
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(kThreads) void short_bwd_kernel(ScanArgs p, const f
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float f, m;
-            sigmoid_pair(xf[t].get(j), f, m);
+            sigmoid_pair<T>(xf[t].get(j), f, m);
             pr[t][j] = c[j] * keep[t];
             c[j] = t < l.len ? f * pr[t][j] + m * xz[t].get(j) : c[j];
         }
@@ -624,8 +624,8 @@ __global__ __launch_bounds__(kThreads) void short_bwd_kernel(ScanArgs p, const f
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float f, m, o, om;
-            sigmoid_pair(xf[t].get(j), f, m);
-            sigmoid_pair(xo[t].get(j), o, om);
+            sigmoid_pair<T>(xf[t].get(j), f, m);
+            sigmoid_pair<T>(xo[t].get(j), o, om);
             const float z = xz[t].get(j), od = o * (dh ? d[t].get(j) : 0.0f), D = od + E[j];
             vf[j] = on ? D * (pr[t][j] - z) * (f * m) : 0.0f;
             vz[j] = on ? D * m : 0.0f;
@@ -653,11 +653,11 @@ __global__ __launch_bounds__(kThreads) void step_kernel(int64_t rows, int64_t U,
     const int64_t i = id / U, u = id - i * U;
     const T* g = gates + i * gr + u;
     float f, b;
-    sigmoid_pair((float)g[0], f, b);
+    sigmoid_pair<T>((float)g[0], f, b);
     const float p = keep ? c[id] * keep[i] : c[id];
     const float now = f * p + b * (float)g[U];
     c_out[id] = now;
-    h[id] = (T)(sigmoid((float)g[2 * U]) * now);
+    h[id] = (T)(sigmoid<T>((float)g[2 * U]) * now);
 }
 
 // Vectors of kWide channels; sequences narrower than that go channel by channel.

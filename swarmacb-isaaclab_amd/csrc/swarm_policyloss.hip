@@ -38,8 +38,6 @@ constexpr float kBound = 20.0f;       // bound of the log-ratios
 constexpr float kInactive = -1.0f;    // s of a row that takes no part (s >= 1 elsewhere: e = 1 at the maximum)
 constexpr unsigned kCountHere = 256;  // up to this many workgroups, each counts the active rows itself
 
-constexpr float kLn2 = 0.69314718055994530942f;
-
 __device__ __forceinline__ float exponent(float z, float m) { return fmaxf((z - m) * kLog2e, -200.0f); }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
