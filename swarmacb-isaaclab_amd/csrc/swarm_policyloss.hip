@@ -1,12 +1,12 @@
 // swarm_policyloss.hip — log-probabilities and the clipped policy loss with a KL term, from logits
 // (include/swarmseq.h: swarm_log_probs, swarm_policy_loss_*).
 //
-// Per row of K logits z with the taken action a, m = max z, x_k = (z_k - m) log2 e, e_k = 2^x_k, s = sum e_k,
+// Per row of K logits z with the taken action a, m = max z, x_k = z_k - m, e_k = exp x_k, s = sum e_k,
 // t = sum e_k x_k:
-//   log p_k = x_k ln 2 - log s,  p_k = e_k / s,  l = log p_a,  H = log s - (t / s) ln 2
+//   log p_k = x_k - log s,  p_k = e_k / s,  l = log p_a,  H = log s - t / s
 //   dz_k = c [ g (1[k = a] - p_k) + entropy_coef p_k (log p_k + H) ],   c = incoming gradient / denominator,
 //   g = d pg / d l + kl_coef (1 - exp(ref - l)).
-// x is held above -200, where e is 0 in float32: a logit of -inf adds nothing to either sum and has no gradient. A
+// x is held above -138, where e is 0 in float32: a logit of -inf adds nothing to either sum and has no gradient. A
 // NaN or an infinite maximum would be lost there, so such a row's s is set to NaN.
 //
 // Memory bound. A row is read once and held in registers by as many threads as it needs; maximum, then both sums,
@@ -38,9 +38,16 @@ constexpr float kBound = 20.0f;       // bound of the log-ratios
 constexpr float kInactive = -1.0f;    // s of a row that takes no part (s >= 1 elsewhere: e = 1 at the maximum)
 constexpr unsigned kCountHere = 256;  // up to this many workgroups, each counts the active rows itself
 
-__device__ __forceinline__ float exponent(float z, float m) { return fmaxf((z - m) * kLog2e, -200.0f); }
+__device__ __forceinline__ float exponent(float z, float m) { return fmaxf(z - m, -138.0f); }
 
-__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+// e of an exponent, of T's logits: good to 3 + |x| / 20 units of 2^-24 in float32, else to 2 + |x|. (float32 with and
+// without the remainder: loss of 5000 x 30000 269 against 264 us, 20000 x 5000 187 against 182. For 16 bits, whose logits'
+// own steps are far larger, it would cost 103 against 94 us at 100000 x 1000.)
+template <typename T>
+__device__ __forceinline__ float exp_of(float x) {
+    const float h = x * kLog2e;
+    return kExact<T> ? exp_from(h, __builtin_fmaf(h, -kLn2, x)) : __builtin_amdgcn_exp2f(h);
+}
 
 // clamp that keeps a NaN
 __device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return x < lo ? lo : (x > hi ? hi : x); }
@@ -276,7 +283,7 @@ struct Sums {
 
 __device__ __forceinline__ Stats stats_from(const Sums& a) {
     const float s = fabsf(a.m) < INFINITY ? a.s : NAN, log_s = logf(s);
-    return {a.m, s, log_s, log_s - a.t * __builtin_amdgcn_rcpf(s) * kLn2};
+    return {a.m, s, log_s, log_s - a.t * __builtin_amdgcn_rcpf(s)};
 }
 
 // Maximum, then both sums. The longest rows, and all that are not held, gather them in one pass, while their later
@@ -295,7 +302,7 @@ __device__ __forceinline__ Sums sums_of(const R& r, int lane, float* red) {
     auto add = [&](const auto& v) {
 #pragma unroll
         for (unsigned j = 0; j < sizeof(v) / sizeof(float); ++j) {
-            const float x = exponent(v[j], m), e = exp2_of(x);
+            const float x = exponent(v[j], m), e = exp_of<typename R::T>(x);
             s += e;
             t += e * x;
         }
@@ -306,7 +313,7 @@ __device__ __forceinline__ Sums sums_of(const R& r, int lane, float* red) {
         r.each(lane, add);
     } else {
         auto rescale = [&](float to) {
-            const float x = exponent(m, to), e = exp2_of(x);
+            const float x = exponent(m, to), e = exp_of<typename R::T>(x);
             t = e * (t + x * s);
             s *= e;
             m = to;
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(kJoin) void log_probs_join_kernel(int64_t K, const 
     for (int64_t p = threadIdx.x; p < parts; p += kJoin) top = Maximum{}(top, w[3 * p]);
     top = group_max<kJoin>(top, nullptr);
     for (int64_t p = threadIdx.x; p < parts; p += kJoin) {
-        const float x = exponent(w[3 * p], top), e = exp2_of(x);
+        const float x = exponent(w[3 * p], top), e = exp_of<T>(x);
         s += e * w[3 * p + 1];
         t += e * (w[3 * p + 2] + x * w[3 * p + 1]);
     }
@@ -498,23 +505,24 @@ __device__ __forceinline__ RowTerms terms_of(const LossArgs& p, const RowIn& in,
 }
 
 // p_k c (entropy_coef (log p_k + H) - g) = e_k (c1 x_k + c0): a row's gradient but for its action
+template <typename T>
 struct RowGrad {
     float m, c1, c0;
     __device__ __forceinline__ RowGrad(float m, float s, float log_s, float H, float g, float c, float ent_coef) : m(m) {
         const float share = __builtin_amdgcn_rcpf(s), ce = c * ent_coef;
-        c1 = ce * kLn2 * share;
+        c1 = ce * share;
         c0 = (ce * (H - log_s) - c * g) * share;
     }
     __device__ __forceinline__ float operator()(float z) const {
         const float x = exponent(z, m);
-        return exp2_of(x) * (c1 * x + c0);
+        return exp_of<T>(x) * (c1 * x + c0);
     }
 };
 
 // A row's gradient. The action's element is stored once more, with its own term, by the thread that stored it.
 template <typename R>
 __device__ __forceinline__ void write_grad(const R& r, typename R::T* out, int lane, int64_t K, const Taken& a,
-                                           float more, const RowGrad& f) {
+                                           float more, const RowGrad<typename R::T>& f) {
     r.write(out, lane, K, f);
     if (a.in && lane == R::owner(a.a)) out[a.a] = (typename R::T)(f(a.z) + more);
 }
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(R::kThreads, 4) void loss_rows_kernel(
             row_stats[4 * m + 2] = st.H;
             row_stats[4 * m + 3] = t.g;
         }
-        if (dz) write_grad(r, dz + m * K, lane, K, a, c * t.g, RowGrad(st.m, st.s, st.log_s, st.H, t.g, c, p.ent_coef));
+        if (dz) write_grad(r, dz + m * K, lane, K, a, c * t.g, RowGrad<typename R::T>(st.m, st.s, st.log_s, st.H, t.g, c, p.ent_coef));
     }
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
@@ -636,7 +644,7 @@ __global__ __launch_bounds__(R::kThreads) void loss_bwd_kernel(
         R r;
         r.load(logits + m * ld, lane, K);
         write_grad(r, dz + m * K, lane, K, taken_of(actions, m, logits + m * ld, K), c * gl,
-                   RowGrad(mx, s, logf(s), H, gl, c, ent_coef));
+                   RowGrad<typename R::T>(mx, s, logf(s), H, gl, c, ent_coef));
     }
 }
 

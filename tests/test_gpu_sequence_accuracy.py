@@ -78,3 +78,27 @@ def test_gates_of_a_step(gpu_device):
     _close(call(x, zero, zero, state=one)[1], f, _units(x), "f")
     _close(call(x, one, zero, state=zero)[1], b, _units(x), "1 - f")
     _close(call(wide, zero, x, state=one)[0], f, _units(x), "o")
+
+
+@pytest.mark.parametrize("grad", [1.0, 2.0])
+@pytest.mark.parametrize("K", [2, 65, 700, 5000, 9000, 20000, 40000])
+def test_unlikely_choices(K, grad, gpu_device):
+    """Two choices y apart, the likely one taken: the other's gradient is its probability, down to 1e-37. Beyond the
+    exponential's 3 + y / 20: the sum 1, its reciprocal 2, the ratio 5, three products 3."""
+    M = 300
+    y = -torch.linspace(0.5, 85.0, M)
+    z = torch.full((M, K), -float("inf"))
+    g = torch.Generator().manual_seed(K)
+    at = torch.stack([torch.randperm(K, generator=g)[:2] for _ in range(M)])
+    rows = torch.arange(M)
+    z[rows, at[:, 0]], z[rows, at[:, 1]] = 0.0, y
+    old = -torch.log1p(y.double().exp())
+    leaf = z.to(gpu_device).requires_grad_()
+    loss, _ = _ops().categorical_policy_loss(leaf, at[:, 0].to(gpu_device), old.float().to(gpu_device),
+                                             torch.ones(M, device=gpu_device), denom=torch.ones((), device=gpu_device))
+    (d,) = torch.autograd.grad(loss, leaf, torch.tensor(grad, device=gpu_device))
+    p = torch.sigmoid(y.double())
+    _close(d[rows, at[:, 1]], grad * p, 16 + y.double().abs() / 20, "gradient of the unlikely choice")
+    d = d.detach().clone()
+    d[rows, at[:, 0]], d[rows, at[:, 1]] = 0.0, 0.0
+    assert not d.any()
