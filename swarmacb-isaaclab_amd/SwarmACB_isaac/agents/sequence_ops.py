@@ -295,6 +295,14 @@ def categorical_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_log
                                          _flag(z.device, what))
 
 
+def _plain_kl(d):
+    """exp(d) - d - 1: by its series where d is small and the difference would cancel (float64 needs 16 terms)."""
+    series = torch.ones_like(d)
+    for k in range(18, 2, -1):
+        series = 1.0 + d / k * series
+    return torch.where(d.abs() < 0.5, 0.5 * d * d * series, torch.expm1(d) - d)
+
+
 def _plain_policy_loss(z, a, old, adv, ref, active, denom, lo, hi, kl_coef, entropy_coef):
     if active is not None:
         z, a, old, adv = z[active], a[active], old[active], adv[active]
@@ -306,8 +314,7 @@ def _plain_policy_loss(z, a, old, adv, ref, active, denom, lo, hi, kl_coef, entr
     if ref is None:
         kl = torch.zeros_like(pg)
     else:
-        d = (ref - lp).clamp(-RATIO_BOUND, RATIO_BOUND)
-        kl = d.exp() - d - 1.0
+        kl = _plain_kl((ref - lp).clamp(-RATIO_BOUND, RATIO_BOUND))
     outside = ((r < lo) | (r > hi)).to(pg.dtype)
     terms = torch.stack([v.sum() / n for v in (pg, kl, ent, outside)])
     return terms[0] + kl_coef * terms[1] - entropy_coef * terms[2], terms.detach()

@@ -102,3 +102,28 @@ def test_unlikely_choices(K, grad, gpu_device):
     d = d.detach().clone()
     d[rows, at[:, 0]], d[rows, at[:, 1]] = 0.0, 0.0
     assert not d.any()
+
+
+def test_references_close_by(gpu_device):
+    """kl = exp d - d - 1 and its gradient where d is small, as it is in every update: with one choice left l is 0, so d
+    is the reference itself. 40 units cover exp d - 1 and its difference to d at |d| = 1 / 2, where they cancel most."""
+    d = torch.logspace(-6, 0.5, 80)
+    d = torch.cat([d, -d, torch.zeros(1)])
+    dd = d.double()
+    kl = torch.where(dd.abs() < 1e-2, dd ** 2 * (0.5 + dd * (1 / 6 + dd * (1 / 24 + dd * (1 / 120 + dd / 720)))),
+                     torch.expm1(dd) - dd)
+    row = torch.zeros(1, device=gpu_device)
+    for k in range(len(d)):
+        _, terms = _ops().categorical_policy_loss(torch.zeros(1, 1, device=gpu_device), row.long(), row, row,
+                                                  ref_log_probs=d[k:k + 1].to(gpu_device), kl_coef=1.0)
+        _close(terms[1], kl[k], torch.tensor(40.0), f"kl of {float(d[k])}")
+        assert float(terms[1]) >= 0.0
+    d, dd, M = d[:-1], dd[:-1], len(d) - 1          # without 0, where the other choice's own e^-30 is all there is
+    z = torch.tensor([0.0, -30.0], device=gpu_device).expand(M, 2).clone().requires_grad_()
+    rows = torch.zeros(M, device=gpu_device)
+    loss, _ = _ops().categorical_policy_loss(z, rows.long(), rows, rows, ref_log_probs=d.to(gpu_device), kl_coef=1.0,
+                                             denom=torch.ones((), device=gpu_device))
+    (dz,) = torch.autograd.grad(loss, z)
+    p = torch.sigmoid(torch.tensor(-30.0, dtype=torch.float64))
+    ref = torch.expm1(dd + torch.log1p(torch.tensor(-30.0, dtype=torch.float64).exp())) * p
+    _close(dz[:, 1], ref, 40 + 0 * ref, "gradient of the other choice")

@@ -165,6 +165,33 @@ def test_policy_loss_cpu(K, kind):
     R.check(ent, H, 1e-12 * (1 + H.abs()), "entropy")
 
 
+@pytest.mark.parametrize("dtype,unit", [(torch.float32, 2.0 ** -24), (torch.float64, 2.0 ** -53)])
+def test_references_close_by_cpu(dtype, unit):
+    """kl = exp d - d - 1 and its gradient where d is small. With one choice left l is 0, so d is the reference itself.
+    40 units cover exp d - 1 and its difference to d at |d| = 1 / 2, where they cancel most."""
+    d = torch.logspace(-6, 0.5, 60, dtype=dtype)
+    d = torch.cat([d, -d])
+    n, dd = len(d), d.double()
+    exact, term = torch.zeros_like(dd), dd
+    for k in range(2, 40):
+        term = term * dd / k
+        exact = exact + term
+    z = torch.tensor([0.0, -30.0], dtype=dtype).expand(n, 2).clone().requires_grad_()
+    row = torch.zeros(n, dtype=dtype)
+    one = [float(categorical_policy_loss(torch.zeros(1, 1, dtype=dtype), row[:1].long(), row[:1], row[:1],
+                                         ref_log_probs=d[k:k + 1], kl_coef=1.0)[1][1]) for k in range(n)]
+    assert min(one) > 0.0
+    R.check(torch.tensor(one, dtype=torch.float64), exact, 40 * unit * exact, "kl")
+    loss, _ = categorical_policy_loss(z, row.long(), row, row, ref_log_probs=d, kl_coef=1.0, denom=torch.ones((), dtype=dtype))
+    (dz,) = torch.autograd.grad(loss, z)
+    p = torch.sigmoid(torch.tensor(-30.0, dtype=torch.float64))
+    want = torch.expm1(dd + torch.log1p(torch.tensor(-30.0, dtype=torch.float64).exp())) * p
+    # l = -log(1 + e^-30) moves d by its own rounding: half a step of 1 for the sum and as much for the logarithm, or all
+    # of e^-30 = p where that is less; the gradient's slope in d is exp(d) p
+    moved = min(2 * unit, float(p)) * dd.exp() * p
+    R.check(dz[:, 1], want, 40 * unit * want.abs() + moved, "gradient of the other choice")
+
+
 def test_policy_loss_gradient_by_differences():
     z, a, old, adv, ref = _loss_inputs(5, 6)
     mask = torch.tensor([True, True, False, True, True])
