@@ -16,12 +16,12 @@ if [ -n "$VARIANTS" ]; then
   IFS=';' read -ra VS <<< "$VARIANTS"
   for v in "${VS[@]}"; do
     name=${v%%:*}; flags=${v#*:}
-    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -shared $flags \
+    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -shared $flags \
       -o $OUT/libcritic_$name.so swarm_critic.hip $OUT/stub.cpp &
   done
 else
   for m in ${MASKS:-0 1 2 4 8 16 6}; do
-    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -shared -DRSA_ABLATE=$m \
+    /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -shared -DRSA_ABLATE=$m \
       -o $OUT/libcritic_$m.so swarm_critic.hip $OUT/stub.cpp &
   done
 fi
