@@ -38,7 +38,8 @@ typedef enum {
  * Steps t >= lengths[i] (clamped to [0, T]) are padding: the state stands still, h is 0, and what gates,
  * keep and d_h hold there is not used (NaN included).
  *   gates: element (i, t, c) at gates[i * gates_n + t * gates_t + c]; c0: [n][U] f32 or NULL (zeros);
- *   keep: [n][T] f32 or NULL (ones); lengths: [n] int64 or NULL (T).
+ *   keep: [n][T] f32 within [-1, 1] or NULL (ones; steps are joined by products of f and keep, which larger values
+ *   would carry out of range); lengths: [n] int64 or NULL (T).
  *   h: [n][T][U]; c_last: [n][U] f32, the state behind the last step;
  *   tile_states: [n][SWARM_GATED_TILES(T)][U] f32, the state before every SWARM_GATED_TILE-th step, for the
  *   backward pass (NULL: not kept); work: swarm_gated_scan_workspace(n, T, U) floats (NULL where that is 0). */

@@ -81,8 +81,8 @@ def gated_recurrence(gates: torch.Tensor, state: torch.Tensor | None = None, kee
         c_t = f_t p_t + (1 - f_t) z_t        p_t = keep_{t-1} c_{t-1},  p_0 = state
         h_t = o_t c_t
 
-    state (n, U) float32 (None: zeros); keep (n, T) float32 or bool multiplies the state after step t before
-    step t + 1, as in ``lstm_sequence`` (0 where the episode ended); lengths (n,) int64 or int32: steps from
+    state (n, U) float32 (None: zeros); keep (n, T) float32 within [-1, 1] or bool multiplies the state after step
+    t before step t + 1, as in ``lstm_sequence`` (0 where the episode ended); lengths (n,) int64 or int32: steps from
     lengths[i] on are padding, where the state stands still, h is 0, no gradient flows, and the inputs'
     values are not used. Returns h (n, T, U) in the gates' type and the state (n, U) behind the last step in
     float32. Gradients flow to gates and state."""

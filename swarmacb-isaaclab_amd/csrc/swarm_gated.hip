@@ -21,14 +21,16 @@
 // 128 channels a workgroup were slower as well (64 x 1024 x 2048).
 // Steps that are padding in every sequence of a workgroup are written and not read.
 //
-// Up to kShort steps need no tiles. Few channels (one long sequence) do not fill the card: then the length is split
+// Up to kShort steps need no tiles. Sequences of fewer than four channels go channel by channel, 16 steps
+// a thread, where the forward kernel spills 136 to 140 bytes. Few channels (one long sequence) do not fill the card: then the length is split
 // into chunks as well, a first kernel composes each chunk, and the main kernel's workgroups start from the chunks
 // before theirs: the gates are read twice.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
 //   64 sequences x 1024 steps x 2048 channels, bf16, ragged: forward 204 us, backward 360 us, 4.3 and 4.5 TB/s
 //   1 x 32768 x 1024, bf16: chunks 37 + forward 54 us, chunks 45 + backward 97 us; the main kernels 5.0 and 4.8 TB/s
-//   256 x 4 x 4096, bf16: 12 + 24 us;  one step, 81920 x 64 float32 (step_kernel): 20.5 us, 6.1 TB/s
+//   256 x 4 x 4096, bf16: 12 + 24 us;  one step, 81920 x 64 (step_kernel): float32 20.5 us, 6.1 TB/s,
+//   bf16 and float16 14.5 us, 5.8 TB/s
 #include <type_traits>
 
 #include "swarm_seq.h"
@@ -526,8 +528,10 @@ __global__ __launch_bounds__(kThreads, V == 1 ? 2 : 3) void scan_bwd_kernel(Scan
 }
 
 // Sequences of at most kShort steps: a thread walks its channels through all of them, with every step's loads in
-// flight at once and nothing to join. (With 4096 channels, 256 sequences and 4 steps in bf16 the tile kernels, most
-// of whose threads then have no step, took 88 + 93 us forward and backward.)
+// flight at once and nothing to join. 16 steps fill its registers, and beat the tile kernels, most of whose threads
+// then have no step (us, forward + backward, against tiles): 256 x 16 x 4032 bf16 39 + 68 / 90 + 95, 256 x 12 x 4064 bf16
+// 25 + 57 / 90 + 96, 256 x 16 x 2000 float32 37 + 47 / 53 + 56. From 17 steps on the tiles' time is what it takes: 91 + 96 for
+// 256 x 17 x 4000 bf16.
 constexpr int kShort = 16;
 
 template <typename T, int V>

@@ -13,14 +13,19 @@
 // are reduced over them. Since the denominator does not depend on the logits, the gradient for an incoming gradient
 // of 1 follows at once, from the same registers: reading the logits once and writing their gradient is all the
 // traffic there is. The backward call keeps that gradient if the incoming one is 1, and otherwise forms it again
-// (scaling a rounded gradient would round it twice). Rows that no workgroup holds are read twice.
+// (scaling a rounded gradient would round it twice). Rows that no workgroup holds are read twice. In float32, rows of
+// 8193 to 32768 logits leave 172 bytes a thread to scratch memory, which four waves a SIMD cost.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
-//   loss, 4096 x 50001, bf16, a tenth masked: 213 us, 3.6 TB/s. Some 115 us of that is arithmetic (two exponentials
+// A tenth of the rows is masked in each loss.
+//   loss, 4096 x 50001, bf16: 214 us, 3.6 TB/s. Some 115 us of that is arithmetic (two exponentials
 //     an element), and of rows of 100 KB a CU's registers and LDS hold two: too few for one row's loads to hide the
 //     other's arithmetic altogether. Rows read twice took 290 us, three rows a CU of 256 threads each 247 us.
-//   loss, 100000 x 1000, bf16: 96 us, 4.2 TB/s;  20000 x 5000, bf16: 102 us, 3.9;  10000 x 15000, bf16: 139 us, 4.3;
-//     10000 x 12000, float32: 218 us, 4.4 TB/s
+//   loss, 100000 x 1000, bf16: 96 us, 4.0 TB/s;  20000 x 5000, bf16: 96 us, 4.0;  10000 x 15000, bf16: 128 us, 4.4;
+//     10000 x 12000, float32: 210 us, 4.3 TB/s
+//   the backward call that forms the gradient again (any incoming one but 1), after its forward call: 4096 x 50001, bf16
+//     178 us after 215, float32 384 after 468; 100000 x 1000, bf16 75 after 96; float16, whose forward call forms none,
+//     4096 x 50001 163 after 156, 2048 x 6 3.7 after 4.9
 //   loss, 2048 x 6, float32: 6.6 + 3.2 us, launches and the last sum
 //   log-probabilities, 8192 x 32768, bf16: 99 us, 5.4 TB/s;  81920 x 18, float32: 3.8 us
 #include <type_traits>
@@ -36,7 +41,10 @@ constexpr int kSums = 6;              // pg, kl, H, outside, pg + kl_coef kl - e
 constexpr int kFinish = 256;          // threads of the last sums
 constexpr float kBound = 20.0f;       // bound of the log-ratios
 constexpr float kInactive = -1.0f;    // s of a row that takes no part (s >= 1 elsewhere: e = 1 at the maximum)
-constexpr unsigned kCountHere = 256;  // up to this many workgroups, each counts the active rows itself
+// Up to this many workgroups, each counts the active rows itself, which spares a launch of 2 us and more. It pays while
+// the rows are few, of any length (loss_rows_kernel, us, against a count of its own: 2048 x 6 6.5 / 5.7, 240 x 5000 bf16
+// 9.5 / 8.2), and not for many short ones (16384 x 6 13.6 / 5.8, 65536 x 6 36.9 / 6.5).
+constexpr unsigned kCountHere = 256;
 
 __device__ __forceinline__ float exponent(float z, float m) { return fmaxf(z - m, -138.0f); }
 

@@ -29,8 +29,8 @@ __device__ __forceinline__ float exp_from(float h, float d) {
 }
 
 // Element types whose own rounding does not cover that error. (Bounded by memory in float32, where it costs nothing:
-// 32 x 1000 x 2048, backward 391 us either way. In 16 bits 1 x 32768 x 1024 took 64 + 116 us forward and backward with it
-// against 60 + 108 without, for errors far below the gates' own steps.)
+// 32 x 1000 x 2048, backward 391 us either way. In 16 bits 1 x 32768 x 1024 took 104 + 161 us forward and backward with it
+// against 98 + 151 without, for errors far below the gates' own steps.)
 template <typename T>
 constexpr bool kExact = sizeof(T) == 4;
 
