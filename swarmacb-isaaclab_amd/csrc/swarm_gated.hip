@@ -22,14 +22,16 @@
 // Steps that are padding in every sequence of a workgroup are written and not read.
 //
 // Up to kShort steps need no tiles. Sequences of fewer than four channels go channel by channel, 16 steps
-// a thread, where the forward kernel spills 136 to 140 bytes. Few channels (one long sequence) do not fill the card: then the length is split
+// a thread, where the forward kernel spills 136 to 140 bytes (100000 x 64 x 1 bf16: 74 + 138 us,
+// 0.7 TB/s). Few channels (one long sequence) do not fill the card: then the length is split
 // into chunks as well, a first kernel composes each chunk, and the main kernel's workgroups start from the chunks
 // before theirs: the gates are read twice.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
-//   64 sequences x 1024 steps x 2048 channels, bf16, ragged: forward 204 us, backward 360 us, 4.3 and 4.5 TB/s
-//   1 x 32768 x 1024, bf16: chunks 37 + forward 54 us, chunks 45 + backward 97 us; the main kernels 5.0 and 4.8 TB/s
-//   256 x 4 x 4096, bf16: 12 + 24 us;  one step, 81920 x 64 (step_kernel): float32 20.5 us, 6.1 TB/s,
+//   64 sequences x 1024 steps x 2048 channels, bf16, ragged: forward 205 us, backward 365 us, 4.3 and 4.5 TB/s
+//   1 x 32768 x 1024, bf16: chunks 38 + forward 59 us, chunks 49 + backward 106 us (36 + 53, 44 + 96 at best); the main
+//   kernels 4.6 and 4.4 TB/s
+//   256 x 4 x 4096, bf16: 11 + 24 us;  one step, 81920 x 64 (step_kernel): float32 20.5 us, 6.1 TB/s,
 //   bf16 and float16 14.5 us, 5.8 TB/s
 #include <type_traits>
 

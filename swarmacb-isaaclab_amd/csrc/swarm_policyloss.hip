@@ -18,13 +18,13 @@
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
 // A tenth of the rows is masked in each loss.
-//   loss, 4096 x 50001, bf16: 214 us, 3.6 TB/s. Some 115 us of that is arithmetic (two exponentials
+//   loss, 4096 x 50001, bf16: 214 to 225 us, 3.5 TB/s. Some 115 us of that is arithmetic (two exponentials
 //     an element), and of rows of 100 KB a CU's registers and LDS hold two: too few for one row's loads to hide the
 //     other's arithmetic altogether. Rows read twice took 290 us, three rows a CU of 256 threads each 247 us.
 //   loss, 100000 x 1000, bf16: 96 us, 4.0 TB/s;  20000 x 5000, bf16: 96 us, 4.0;  10000 x 15000, bf16: 128 us, 4.4;
 //     10000 x 12000, float32: 210 us, 4.3 TB/s
 //   the backward call that forms the gradient again (any incoming one but 1), after its forward call: 4096 x 50001, bf16
-//     178 us after 215, float32 384 after 468; 100000 x 1000, bf16 75 after 96; float16, whose forward call forms none,
+//     183 us after 225, float32 384 after 468; 100000 x 1000, bf16 75 after 96; float16, whose forward call forms none,
 //     4096 x 50001 163 after 156, 2048 x 6 3.7 after 4.9
 //   loss, 2048 x 6, float32: 6.6 + 3.2 us, launches and the last sum
 //   log-probabilities, 8192 x 32768, bf16: 99 us, 5.4 TB/s;  81920 x 18, float32: 3.8 us

@@ -10,7 +10,7 @@
 // gradient there; the workgroups' sums are added in a fixed order by a second kernel.
 //
 // Measured (a 4 GiB copy reaches 4.8 TB/s of reads and writes together on this card):
-//   16384 x 4096, bf16: forward 82 us, 6.6 TB/s; backward 139 us, 4.8 TB/s, and 5 us for the weight gradient's last sum
+//   16384 x 4096, bf16: forward 83 us, 6.5 TB/s; backward 139 us, 4.8 TB/s, and 5 us for the weight gradient's last sum
 //   5001 x 1001, float16: 9 us, then 16 + 7 us;  200000 x 512, bf16: 143 and 164 us, 5.7 and 6.2 TB/s
 //   16384 x 4096, float16: 80 us, then 139 + 5 us
 //   4096 x 16384, float32, where the backward pass spills 80 bytes a thread (16 bits: 36 to 44): 250 and 278 us, 4.3 and
